@@ -22,6 +22,8 @@ LIB_PATH = os.environ.get("DLQ_LIB_PATH") or os.path.join(_HERE, "libdlq.so")
 DLQ_OK = 0
 DLQ_OUT_S8, DLQ_OUT_F32, DLQ_OUT_S32 = 0, 1, 2
 DLQ_PREC_INT8, DLQ_PREC_FP8 = 0, 1
+DLQ_T_F32, DLQ_T_BF16 = 0, 1
+DLQ_ACT = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 # kernel families of dlq_resnet18_timing (include/dlq.h DLQ_FAM_*)
 # (the first word names the int8 forward's kernel; the fp8 forward runs
 # stem_fused_kernel and block_l1_kernel in families 0 and 1)
@@ -37,6 +39,10 @@ class DLQError(RuntimeError):
 
 class ConvDesc(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("N", "H", "W", "C", "OC", "kH", "kW", "sH", "sW", "pH", "pW")]
+
+
+class LinearDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("M", "N", "K", "ldx", "ldw", "ldy", "ldr", "act", "out_type")]
 
 
 _vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
@@ -126,6 +132,14 @@ _SIGS = {
     "dlq_stem_fused_f8": ([_vp, _i, _vp, _vp, _vp, _f, _vp, _vp], _i),
     "dlq_conv2d_s2_ds_nhwc_f8": ([C.POINTER(ConvDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp], _i),
     "dlq_block_l1_nhwc_f8": ([_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, C.c_float, _vp, _vp], _i),
+    "dlq_quantize_rows_dyn_s8": ([_vp, _i, _i, _i, _i, _vp, _i, _vp, _vp], _i),
+    "dlq_quantize_rows_dyn_f8": ([_vp, _i, _i, _i, _i, _vp, _i, _vp, _vp], _i),
+    "dlq_linear_act_s8": ([C.POINTER(LinearDesc)] + [_vp] * 8, _i),
+    "dlq_linear_act_f8": ([C.POINTER(LinearDesc)] + [_vp] * 8, _i),
+    "dlq_linear_grouped_s8": ([C.POINTER(LinearDesc), _i] + [_vp] * 9, _i),
+    "dlq_linear_grouped_f8": ([C.POINTER(LinearDesc), _i] + [_vp] * 9, _i),
+    "dlq_logprobs_workspace_bytes": ([_i, _i, _i], _sz),
+    "dlq_logprobs": ([_vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp], _i),
 }
 
 if not os.path.exists(LIB_PATH):

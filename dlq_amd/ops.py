@@ -13,12 +13,13 @@ Like the reference helpers they raise on failure instead of returning codes
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import numpy as np
 import torch
 
-from .lib import (DLQ_OUT_F32, DLQ_OUT_S8, DLQ_OUT_S32, ConvDesc, check, lib, ptr,
-                  stream_handle)
+from .lib import (DLQ_ACT, DLQ_OUT_F32, DLQ_OUT_S8, DLQ_OUT_S32, DLQ_T_BF16, DLQ_T_F32, ConvDesc, LinearDesc,
+                  check, lib, ptr, stream_handle)
 
 
 def out_dim(n, k, s, p):
@@ -442,3 +443,177 @@ def block_l1_f8(x: torch.Tensor, w1: torch.Tensor, alpha1: torch.Tensor, beta1: 
     check(lib.dlq_block_l1_nhwc_f8(ptr(x), x.shape[0], ptr(w1), ptr(alpha1), ptr(beta1), ptr(w2), ptr(alpha2),
                                    ptr(beta2), float(res_scale), ptr(y), stream_handle()), "block_l1_f8")
     return y
+
+
+# ------------------------------------------- row operators (tokens as rows)
+# include/dlq.h "Row operators of quantised transformer serving".  Tensors may
+# be row-strided views (unit stride within a row); all of a call's tensors lie
+# on one device, which need not be the current one; the work goes to that
+# device's current stream.
+
+_TYPES = {torch.float32: DLQ_T_F32, torch.bfloat16: DLQ_T_BF16}
+
+
+def _rows(t: torch.Tensor, name: str, dtypes, rows=None, cols=None) -> int:
+    """Checks a row-strided CUDA matrix; its row stride in elements."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
+        raise TypeError(f"{name}: expected a CUDA tensor of {' or '.join(map(str, dtypes))}")
+    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [{'rows' if rows is None else rows}, "
+                         f"{'cols' if cols is None else cols}]")
+    r, c = t.shape
+    ld = t.stride(0) if r > 1 else c
+    if (c > 1 and t.stride(1) != 1) or ld < c:
+        raise ValueError(f"{name}: rows must have unit stride and not overlap, strides {t.stride()}")
+    return ld
+
+
+def _vector(t, name: str, dtype, shape):
+    """Checks an optional contiguous CUDA tensor; its address or None."""
+    if t is None:
+        return None
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.is_contiguous()):
+        raise TypeError(f"{name}: expected a contiguous CUDA tensor of {dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return t.data_ptr()
+
+
+def _launch(what: str, fn, tensors, *args) -> None:
+    """fn(*args, stream) on the tensors' one device and its current stream."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    if dev.index == torch.cuda.current_device():
+        check(fn(*args, stream_handle()), what)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, stream_handle()), what)
+
+
+def _quantize_rows_dyn(what, fn, dtype, x, ld):
+    ldx = _rows(x, "x", _TYPES)
+    rows, cols = x.shape
+    q = torch.empty((rows, cols if ld is None else ld), dtype=dtype, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _launch(what, fn, (x,), x.data_ptr(), _TYPES[x.dtype], rows, cols, ldx, q.data_ptr(), q.shape[1],
+            scale.data_ptr())
+    return q, scale
+
+
+def quantize_rows_dyn_s8(x: torch.Tensor, ld: int | None = None):
+    """fp32 / bf16 rows [rows, cols] -> (int8 codes [rows, ld], fp32 scale
+    [rows]): every row at its own scale max|x|/127 (dlq_quantize_rows_dyn_s8);
+    columns cols..ld-1 zero."""
+    return _quantize_rows_dyn("quantize_rows_dyn_s8", lib.dlq_quantize_rows_dyn_s8, torch.int8, x, ld)
+
+
+def quantize_rows_dyn_f8(x: torch.Tensor, ld: int | None = None):
+    """e4m3 twin of quantize_rows_dyn_s8: uint8 codes at max|x|/448 per row."""
+    return _quantize_rows_dyn("quantize_rows_dyn_f8", lib.dlq_quantize_rows_dyn_f8, torch.uint8, x, ld)
+
+
+def _linear(what, fn, code, x, w, x_scale, w_scale, bias, act, residual, out_dtype, out, offsets=None):
+    if act not in DLQ_ACT:
+        raise ValueError(f"act must be one of {sorted(DLQ_ACT)}, got {act!r}")
+    if out is not None:
+        out_dtype = out.dtype
+    if out_dtype not in _TYPES:
+        raise TypeError("output must be torch.float32 or torch.bfloat16")
+    ldx = _rows(x, "x", (code,))
+    M, K = x.shape
+    if offsets is None:
+        ldw = _rows(w, "w", (code,), cols=K)
+        N, lead = w.shape[0], ()
+    else:
+        if not (isinstance(w, torch.Tensor) and w.is_cuda and w.dtype == code and w.dim() == 3 and w.is_contiguous()):
+            raise TypeError(f"w: expected a contiguous CUDA tensor [E, N, K] of {code}")
+        E, N, ldw = w.shape
+        lead = (E,)
+        if ldw != K:
+            raise ValueError(f"w: shape {tuple(w.shape)}, expected [E, N, {K}]")
+    if w_scale is None:
+        raise TypeError("w_scale is required")
+    sx = _vector(x_scale, "x_scale", torch.float32, (M,))
+    sw = _vector(w_scale, "w_scale", torch.float32, lead + (N,))
+    sb = _vector(bias, "bias", torch.float32, lead + (N,))
+    ldr = 0 if residual is None else _rows(residual, "residual", (out_dtype,), M, N)
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    d = LinearDesc(M, N, K, ldx, ldw, _rows(out, "out", (out_dtype,), M, N), ldr, DLQ_ACT[act], _TYPES[out_dtype])
+    args = (x.data_ptr(), sx, w.data_ptr(), sw, sb, None if residual is None else residual.data_ptr(), out.data_ptr())
+    if offsets is not None:
+        args = (E, _vector(offsets, "offsets", torch.int32, (E + 1,))) + args
+    _launch(what, fn, (x, w, x_scale, w_scale, bias, residual, out, offsets), C.byref(d), *args)
+    return out
+
+
+def linear_act_s8(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None, w_scale: torch.Tensor,
+                  bias: torch.Tensor | None = None, act: str = "none", residual: torch.Tensor | None = None,
+                  out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
+    """act((x @ w.T) * x_scale[:, None] * w_scale + bias) + residual on int8
+    codes x[M, K], w[N, K] (dlq_linear_act_s8): [M, N] fp32 or bf16, rounded
+    once.  act: "none", "relu", "gelu", "gelu_tanh", "silu".  `out` receives the
+    result if given; `residual` may be `out`."""
+    return _linear("linear_act_s8", lib.dlq_linear_act_s8, torch.int8, x, w, x_scale, w_scale, bias, act, residual,
+                   out_dtype, out)
+
+
+def linear_act_f8(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None, w_scale: torch.Tensor,
+                  bias: torch.Tensor | None = None, act: str = "none", residual: torch.Tensor | None = None,
+                  out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
+    """e4m3 twin of linear_act_s8 (uint8 codes)."""
+    return _linear("linear_act_f8", lib.dlq_linear_act_f8, torch.uint8, x, w, x_scale, w_scale, bias, act, residual,
+                   out_dtype, out)
+
+
+def linear_grouped_s8(x: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None,
+                      w_scale: torch.Tensor, bias: torch.Tensor | None = None, act: str = "none",
+                      residual: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float32,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """linear_act_s8 with an expert's weights for each row: rows
+    offsets[e]..offsets[e+1]-1 of x[T, K] (offsets int32 [E+1] on the device,
+    rows sorted by expert) take w[e] of w[E, N, K], w_scale[e] and bias[e]
+    (dlq_linear_grouped_s8).  Rows outside every expert's range are not
+    written: they hold what `out` held (undefined without `out`)."""
+    if offsets is None:
+        raise TypeError("offsets is required")
+    return _linear("linear_grouped_s8", lib.dlq_linear_grouped_s8, torch.int8, x, w, x_scale, w_scale, bias, act,
+                   residual, out_dtype, out, offsets)
+
+
+def linear_grouped_f8(x: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None,
+                      w_scale: torch.Tensor, bias: torch.Tensor | None = None, act: str = "none",
+                      residual: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float32,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """e4m3 twin of linear_grouped_s8 (uint8 codes)."""
+    if offsets is None:
+        raise TypeError("offsets is required")
+    return _linear("linear_grouped_f8", lib.dlq_linear_grouped_f8, torch.uint8, x, w, x_scale, w_scale, bias, act,
+                   residual, out_dtype, out, offsets)
+
+
+class LogProbs(NamedTuple):
+    logprob: torch.Tensor | None      # [rows] fp32, of the given tokens
+    entropy: torch.Tensor             # [rows] fp32
+    top_idx: torch.Tensor | None      # [rows, top] int32
+    top_logprob: torch.Tensor | None  # [rows, top] fp32
+
+
+def logprobs(x: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0) -> LogProbs:
+    """Log probabilities of fp32 / bf16 logits [rows, K] (dlq_logprobs): of
+    tokens int32 [rows] (0 where negative), the rows' entropy, and the `top`
+    (<= 64) largest with their indices, equal ones by ascending index."""
+    ldx = _rows(x, "x", _TYPES)
+    rows, K = x.shape
+    t = _vector(tokens, "tokens", torch.int32, (rows,))
+    lp = None if tokens is None else torch.empty(rows, dtype=torch.float32, device=x.device)
+    ent = torch.empty(rows, dtype=torch.float32, device=x.device)
+    ti = torch.empty((rows, top), dtype=torch.int32, device=x.device) if top > 0 else None
+    tl = torch.empty((rows, top), dtype=torch.float32, device=x.device) if top > 0 else None
+    nb = lib.dlq_logprobs_workspace_bytes(rows, K, top)
+    ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
+    _launch("logprobs", lib.dlq_logprobs, (x, tokens), x.data_ptr(), _TYPES[x.dtype], rows, K, ldx, t, top, ptr(lp),
+            ent.data_ptr(), ptr(ti), ptr(tl), ptr(ws), nb)
+    return LogProbs(lp, ent, ti, tl)

@@ -505,6 +505,90 @@ int dlq_linear_f8(const uint8_t* x, int N, int K, const uint8_t* w, int O, const
 #define DLQ_PREC_FP8 1
 int dlq_resnet18_set_precision(dlq_resnet18* m, int precision);
 
+/* ------------------------------------------------------------------------ */
+/* Row operators of quantised transformer serving.  No reference code exists */
+/* for them; they stand beside dlq_quantize_rows_s8, dlq_linear_s8,          */
+/* dlq_linear_f8, dlq_softmax_f32 and dlq_top1_f32.  Rows are tokens; every  */
+/* matrix is row-major with a row stride ("ld", in elements) of its own and  */
+/* any base alignment its element type allows (16-byte aligned bases and     */
+/* strides that are multiples of 16 bytes run fastest).  Forward only.  The  */
+/* current device must be the stream's.                                      */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of rows that are not codes. */
+#define DLQ_T_F32 0
+#define DLQ_T_BF16 1
+
+/* One scale per row, found and applied in one call:
+ *   a = max_k |x[r][k]|,  scale[r] = a / m (m = 127, e4m3: 448),
+ *   q[r][k] = rne(clamp(x[r][k] * (1 / scale[r]), +-m))  (fp32 IEEE steps).
+ * A row with a < 2^-100 counts as zero: scale 1, codes 0.  A row holding an
+ * infinity or a NaN gets scale NaN and codes 0, so that every product with it
+ * is NaN.  Columns cols..ldq-1 of q are written as zero.  x: rows x cols of
+ * x_type at row stride ldx.  x and q must not overlap. */
+int dlq_quantize_rows_dyn_s8(const void* x, int x_type, int rows, int cols, int ldx, int8_t* q, int ldq, float* scale,
+                             void* stream);
+int dlq_quantize_rows_dyn_f8(const void* x, int x_type, int rows, int cols, int ldx, uint8_t* q, int ldq, float* scale,
+                             void* stream);
+
+/* Activations of the products' epilogue. */
+#define DLQ_ACT_NONE 0
+#define DLQ_ACT_RELU 1
+#define DLQ_ACT_GELU 2      /* v/2 (1 + erf(v/sqrt 2))                          */
+#define DLQ_ACT_GELU_TANH 3 /* v/2 (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3)))    */
+#define DLQ_ACT_SILU 4      /* v / (1 + e^-v)                                   */
+
+typedef struct dlq_linear_desc {
+  int M, N, K;            /* rows of x, rows of w (output columns), contraction */
+  int ldx, ldw, ldy, ldr; /* row strides in elements (ldr read if residual)     */
+  int act;                /* DLQ_ACT_*                                          */
+  int out_type;           /* DLQ_T_F32 or DLQ_T_BF16: y and residual            */
+} dlq_linear_desc;
+
+/* y[m][n] = act(v) + residual[m][n], rounded once to out_type, with
+ *   v = fma(float(acc), x_scale[m] * w_scale[n], bias[n]),
+ *   acc = sum_k x[m][k] * w[n][k]
+ * (s8: the exact int32 sum; e4m3: exact products summed in fp32, in a fixed
+ * order).  x_scale, bias and residual may be NULL (1, 0, none); w_scale not.
+ * w is used as stored: no packing.  residual may be y itself (same ld); any
+ * other overlap of y with an input is not allowed.  K <= 131071 (an int32 sum
+ * of 2^14-sized products); K = 0 gives acc = 0. */
+int dlq_linear_act_s8(const dlq_linear_desc* d, const int8_t* x, const float* x_scale, const int8_t* w,
+                      const float* w_scale, const float* bias, const void* residual, void* y, void* stream);
+int dlq_linear_act_f8(const dlq_linear_desc* d, const uint8_t* x, const float* x_scale, const uint8_t* w,
+                      const float* w_scale, const float* bias, const void* residual, void* y, void* stream);
+
+/* The same product for rows sorted by expert: rows offsets[e] <= t <
+ * offsets[e+1] use w[e], w_scale[e], bias[e] (w[E][N][ldw], w_scale and
+ * bias[E][N]).  offsets[E+1] lies on the device (non-decreasing, within 0..M;
+ * others are clamped into that range, never read or written beyond it).  Rows
+ * of y before offsets[0] and from offsets[E] on are left as they were; experts
+ * without a row cost nothing.  d->M: rows of x and y.  E <= 65535. */
+int dlq_linear_grouped_s8(const dlq_linear_desc* d, int E, const int32_t* offsets, const int8_t* x,
+                          const float* x_scale, const int8_t* w, const float* w_scale, const float* bias,
+                          const void* residual, void* y, void* stream);
+int dlq_linear_grouped_f8(const dlq_linear_desc* d, int E, const int32_t* offsets, const uint8_t* x,
+                          const float* x_scale, const uint8_t* w, const float* w_scale, const float* bias,
+                          const void* residual, void* y, void* stream);
+
+/* Log probabilities of rows of K logits (fp32 or bf16, row stride ldx):
+ *   lp[j] = x[j] - max - log S,  S = sum_j e^(x[j] - max),
+ *   logprob[r] = lp[tokens[r]] (0 where tokens[r] < 0: no token given; NaN
+ *   where tokens[r] >= K),  entropy[r] = -sum_j e^lp[j] lp[j],
+ *   top_idx / top_logprob[r][0..top): the `top` largest logits in descending
+ *   order, equal ones by ascending index (NaN counts as the largest).
+ * Sums in fp32.  Logits of -inf (masked) have probability 0; a row of nothing
+ * else has logprob -inf, entropy 0 and alternatives 0, 1, ... at -inf.  A NaN
+ * or +inf in a row makes its logprob, entropy and top_logprob NaN.  tokens
+ * and logprob come together or are both NULL; entropy may be NULL; 0 <= top
+ * <= min(64, K), 0: top_idx and top_logprob unused.
+ * workspace: dlq_logprobs_workspace_bytes(rows, K, top) device bytes, 8-byte
+ * aligned, for this call alone while it runs (0 bytes: may be NULL). */
+size_t dlq_logprobs_workspace_bytes(int rows, int K, int top);
+int dlq_logprobs(const void* x, int x_type, int rows, int K, int ldx, const int32_t* tokens, int top, float* logprob,
+                 float* entropy, int32_t* top_idx, float* top_logprob, void* workspace, size_t ws_bytes,
+                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,637 @@
+"""GPU: the row operators against plain 64-bit forms.
+
+Tolerances (u = 2^-24, the half step of fp32; bf16's is 2^-8):
+ * products: the int8 sum is exact, float() of it, x_scale * w_scale and the
+   fma round once each: |dv| <= u (2 |acc s| + |v|).  The activations' slopes
+   stay below 1.13 and their own evaluation (erf, exp, the argument's few
+   products) is off by at most 8 u |v|; the residual's add and the output's
+   rounding are half a step each.  e4m3: products are exact and fp32 sums of K
+   of them take K/32 matrix steps of up to 32 additions' depth and the join of
+   at most 16 slices, so (K/32 + 48) u sum |x w| more.
+ * codes and scales are compared exactly: every step is one IEEE operation.
+ * log probabilities: see lp_bounds.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HALF = {torch.float32: U, torch.bfloat16: 2.0 ** -8}
+F8 = torch.float8_e4m3fn
+ACTS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
+
+
+def codes(rng, t, *shape):
+    x = rng.standard_normal(shape)
+    if t == "s8":
+        return torch.from_numpy(np.clip(np.rint(x * 40), -127, 127).astype(np.int8))
+    return torch.from_numpy(x.astype(np.float32) * 100).clamp(-448, 448).to(F8).view(torch.uint8)
+
+
+def values(q):
+    return q.double() if q.dtype == torch.int8 else q.view(F8).double()
+
+
+def act64(v, act):
+    if act == "relu":
+        return torch.relu(v)
+    if act == "gelu":
+        return v * torch.special.ndtr(v)
+    if act == "gelu_tanh":
+        return 0.5 * v * (1 + torch.tanh(math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)))
+    return v * torch.sigmoid(v) if act == "silu" else v
+
+
+def product64(x, w, xs, ws, bias, act, res, out_dtype):
+    """(y, tolerance) in 64 bits on the CPU."""
+    vx, vw = values(x), values(w)
+    s = (1.0 if xs is None else xs.double()[:, None]) * ws.double()
+    acc = vx @ vw.T * s
+    v = acc if bias is None else acc + bias.double()
+    y = act64(v, act)
+    if res is not None:
+        y = y + res.double()
+    tol = 1.13 * U * (2 * acc.abs() + v.abs()) + 8 * U * v.abs() + U * y.abs() + 1e-30
+    if x.dtype == torch.uint8:
+        tol = tol + 1.13 * U * (x.shape[1] / 32 + 48) * (vx.abs() @ vw.abs().T) * s
+    return y, tol + HALF[out_dtype] * (y.abs() + tol)
+
+
+def close(got, ref, tol, what=""):
+    d = (got.double().cpu() - ref).abs()
+    bad = ~(d <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((d / tol).max()):.3g} x the bound"
+
+
+def strided(t, pad, fill=0):
+    """The same rows cut from a wider device buffer."""
+    big = torch.full((t.shape[0], t.shape[1] + pad), fill, dtype=t.dtype, device="cuda")
+    big[:, :t.shape[1]] = t.cuda()
+    return big[:, :t.shape[1]]
+
+
+def linear(t):
+    from dlq_amd import ops
+    return (ops.linear_act_s8, ops.linear_grouped_s8) if t == "s8" else (ops.linear_act_f8, ops.linear_grouped_f8)
+
+
+def case(rng, t, M, N, K, out, bias=True, res=True, xs=True):
+    x, w = codes(rng, t, M, K), codes(rng, t, N, K)
+    f = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32))  # noqa: E731
+    one = (1 / 40 if t == "s8" else 1 / 100)
+    return dict(x=x, w=w, xs=torch.exp(f(M) * 0.3) * one if xs else None,
+                ws=torch.exp(f(N) * 0.3) * one / max(K, 1) ** 0.5 * (1 if xs else one),
+                bias=f(N) if bias else None, res=f(M, N).to(out) if res else None)
+
+
+def dev(t):
+    return None if t is None else t.cuda()
+
+
+SHAPES = [(1, 1, 1), (1, 16, 64), (1, 4096, 512), (3, 17, 31), (2, 129, 1000), (16, 48, 128), (17, 64, 129),
+          (33, 100, 255), (64, 128, 1024), (65, 257, 300), (128, 128, 256), (100, 1000, 512), (130, 384, 640),
+          (257, 260, 1040), (300, 513, 144), (512, 512, 2048)]
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_linear_shapes(gpu, t, M, N, K, out):
+    rng = np.random.default_rng([M, N, K])
+    c = case(rng, t, M, N, K, out)
+    act = ACTS[(M + N + K) % 5]
+    got = linear(t)[0](dev(c["x"]), dev(c["w"]), dev(c["xs"]), dev(c["ws"]), dev(c["bias"]), act, dev(c["res"]), out)
+    close(got, *product64(**c, act=act, out_dtype=out), f"{M}x{N}x{K}")
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("bias,res,xs", [(0, 0, 0), (1, 0, 1), (0, 1, 1), (1, 1, 0)])
+def test_linear_epilogue(gpu, t, act, bias, res, xs):
+    rng = np.random.default_rng(5)
+    for M, N, K in ((5, 70, 200), (150, 200, 256)):
+        c = case(rng, t, M, N, K, torch.float32, bias, res, xs)
+        got = linear(t)[0](dev(c["x"]), dev(c["w"]), dev(c["xs"]), dev(c["ws"]), dev(c["bias"]), act, dev(c["res"]))
+        close(got, *product64(**c, act=act, out_dtype=torch.float32))
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("M,N,K", [(1, 100, 100), (9, 80, 333), (70, 200, 161), (200, 300, 160), (260, 520, 336)])
+@pytest.mark.parametrize("px,pw,py,pr", [(1, 3, 5, 7), (16, 16, 4, 4), (48, 0, 16, 0), (7, 16, 1, 8)])
+def test_linear_strides(gpu, t, M, N, K, px, pw, py, pr):
+    """Rows cut from wider buffers: the codes beside them are NaN (e4m3) or
+    large, the cells beside y's rows stay as they were."""
+    rng = np.random.default_rng([M, px])
+    out = torch.bfloat16
+    c = case(rng, t, M, N, K, out)
+    wide = torch.full((M, N + py), 3.0, dtype=out, device="cuda")
+    y = wide[:, :N]
+    got = linear(t)[0](strided(c["x"], px, 0x7F), strided(c["w"], pw, 0x7F), dev(c["xs"]), dev(c["ws"]),
+                       dev(c["bias"]), "silu", strided(c["res"], pr), out=y)
+    assert got is y
+    close(y, *product64(**c, act="silu", out_dtype=out))
+    assert (wide[:, N:] == 3.0).all()
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+def test_linear_unaligned_bases(gpu, t):
+    """Every operand at an odd multiple of its element size."""
+    rng = np.random.default_rng(8)
+    M, N, K = 40, 72, 256
+    c = case(rng, t, M, N, K, torch.float32)
+
+    def at(v, skip):
+        b = torch.zeros(v.numel() + skip, dtype=v.dtype, device="cuda")[skip:]
+        return b.copy_(v.reshape(-1)).view(v.shape)
+
+    for skip in (1, 3):
+        got = linear(t)[0](at(c["x"], skip), at(c["w"], skip), at(c["xs"], skip), at(c["ws"], skip),
+                           at(c["bias"], skip), "gelu", at(c["res"], skip),
+                           out=at(torch.zeros(M, N), skip))
+        close(got, *product64(**c, act="gelu", out_dtype=torch.float32))
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("M", [3, 300])
+def test_linear_residual_in_place(gpu, t, M):
+    rng = np.random.default_rng(9)
+    c = case(rng, t, M, 320, 256, torch.bfloat16)
+    y = dev(c["res"])
+    linear(t)[0](dev(c["x"]), dev(c["w"]), dev(c["xs"]), dev(c["ws"]), None, "relu", y, out=y)
+    close(y, *product64(**(c | dict(bias=None)), act="relu", out_dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+def test_linear_no_contraction_and_nan_scale(gpu, t):
+    x = torch.zeros(5, 0, dtype=torch.int8 if t == "s8" else torch.uint8, device="cuda")
+    w = torch.zeros(9, 0, dtype=x.dtype, device="cuda")
+    b = torch.randn(9, device="cuda")
+    y = linear(t)[0](x, w, None, torch.ones(9, device="cuda"), b)
+    assert torch.equal(y, b.expand(5, 9))
+    rng = np.random.default_rng(2)
+    c = case(rng, t, 6, 20, 64, torch.float32, True, False)
+    c["xs"][3] = math.nan  # a row that quantize_rows_dyn found an infinity in
+    y = linear(t)[0](dev(c["x"]), dev(c["w"]), dev(c["xs"]), dev(c["ws"]), dev(c["bias"]), "relu").cpu()
+    assert y[3].isnan().all() and not y[[0, 1, 2, 4, 5]].isnan().any()
+
+
+def test_linear_extreme_codes(gpu):
+    """The largest int8 sums: -128 * -128 * 131071 is below 2^31."""
+    from dlq_amd import ops
+    K = 131071
+    x = torch.full((2, K), -128, dtype=torch.int8, device="cuda")
+    x[1] = 127
+    w = torch.full((33, K), -128, dtype=torch.int8, device="cuda")
+    y = ops.linear_act_s8(x, w, None, torch.ones(33, device="cuda")).cpu()
+    assert (y[0] == float(np.float32(16384 * K))).all() and (y[1] == float(np.float32(-16256 * K))).all()
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+def test_linear_offsets_past_32_bits(gpu, t):
+    """Rows 1.5 GB apart: their byte offsets pass 2^32."""
+    rng = np.random.default_rng(4)
+    M, N, K, ld = 4, 40, 160, 1_500_000_000
+    c = case(rng, t, M, N, K, torch.float32)
+    big = torch.empty(3 * ld + K, dtype=c["x"].dtype, device="cuda")
+    x = big.as_strided((M, K), (ld, 1))
+    x.copy_(c["x"])
+    got = linear(t)[0](x, dev(c["w"]), dev(c["xs"]), dev(c["ws"]), dev(c["bias"]), "none", dev(c["res"]))
+    close(got, *product64(**c, act="none", out_dtype=torch.float32))
+    del big, x
+    torch.cuda.empty_cache()
+
+
+def grouped_reference(c, off, t, act, out, T):
+    y = torch.full((T, c["w"].shape[1]), 3.0, dtype=torch.float64)
+    tol = torch.zeros_like(y)
+    for e in range(len(off) - 1):
+        lo, hi = off[e], off[e + 1]
+        if lo < hi:
+            y[lo:hi], tol[lo:hi] = product64(c["x"][lo:hi], c["w"][e], c["xs"][lo:hi], c["ws"][e],
+                                             None if c["bias"] is None else c["bias"][e], act,
+                                             None if c["res"] is None else c["res"][lo:hi], out)
+    return y, tol
+
+
+def grouped_case(rng, t, E, T, N, K, out, bias=True, res=True):
+    c = case(rng, t, T, N, K, out, bias, res)
+    c["w"] = codes(rng, t, E, N, K)
+    c["ws"] = c["ws"] * torch.from_numpy(rng.uniform(0.5, 2, (E, 1)).astype(np.float32))
+    if bias:
+        c["bias"] = torch.from_numpy(rng.standard_normal((E, N)).astype(np.float32))
+    return c
+
+
+GROUPS = [  # offsets, rows of x
+    ([0, 1], 1), ([0, 0, 3], 3), ([0, 5, 5, 5, 40], 40), ([2, 10, 11, 30], 33), ([0, 0, 0], 4),
+    ([0, 16, 32, 33, 200], 200), ([0, 130, 131, 260, 300], 301), ([0, 300, 300, 301], 310),
+]
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("N,K", [(17, 65), (96, 128), (260, 400)])
+@pytest.mark.parametrize("off,T", GROUPS, ids=[str(g[0]) for g in GROUPS])
+def test_grouped(gpu, t, N, K, off, T):
+    rng = np.random.default_rng([T, N])
+    out = torch.bfloat16 if N == 96 else torch.float32
+    c = grouped_case(rng, t, len(off) - 1, T, N, K, out)
+    y = torch.full((T, N), 3.0, dtype=out, device="cuda")  # rows of no expert keep this
+    o = torch.tensor(off, dtype=torch.int32, device="cuda")
+    linear(t)[1](dev(c["x"]), o, dev(c["w"]), dev(c["xs"]), dev(c["ws"]), dev(c["bias"]), "silu", dev(c["res"]), out=y)
+    close(y, *grouped_reference(c, off, t, "silu", out, T))
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("E,T", [(64, 64), (200, 333), (129, 2000), (3, 1500)])
+def test_grouped_many(gpu, t, E, T):
+    rng = np.random.default_rng([E, T])
+    N, K = 80, 192
+    cut = np.sort(rng.integers(0, T + 1, E - 1))
+    off = [0, *cut.tolist(), T - T // 10]
+    off = [min(o, off[-1]) for o in off]
+    c = grouped_case(rng, t, E, T, N, K, torch.float32, res=False)
+    y = torch.full((T, N), 3.0, device="cuda")
+    linear(t)[1](dev(c["x"]), torch.tensor(off, dtype=torch.int32, device="cuda"), dev(c["w"]), dev(c["xs"]),
+                 dev(c["ws"]), dev(c["bias"]), "gelu_tanh", out=y)
+    close(y, *grouped_reference(c, off, t, "gelu_tanh", torch.float32, T))
+
+
+def test_grouped_offsets_outside(gpu):
+    """Offsets beyond the rows are taken as the nearest row; nothing else is touched."""
+    from dlq_amd import ops
+    rng = np.random.default_rng(3)
+    T, N, K = 40, 64, 128
+    c = grouped_case(rng, "s8", 3, T, N, K, torch.float32, res=False)
+    buf = torch.full((T + 8, N), 3.0, device="cuda")
+    y = buf[4:4 + T]
+    off = torch.tensor([-7, 10, 30, 2_000_000_000], dtype=torch.int32, device="cuda")
+    ops.linear_grouped_s8(dev(c["x"]), off, dev(c["w"]), dev(c["xs"]), dev(c["ws"]), dev(c["bias"]), out=y)
+    close(y, *grouped_reference(c, [0, 10, 30, T], "s8", "none", torch.float32, T))
+    assert (buf[:4] == 3.0).all() and (buf[4 + T:] == 3.0).all()
+
+
+# ------------------------------------------------------------- quantisation
+
+def quant_reference(x, t, ld):
+    m = np.float32(127 if t == "s8" else 448)
+    v = x.float().numpy()
+    a = np.abs(v).max(1)
+    bad = ~np.isfinite(a)
+    zero = ~bad & (a < 2.0 ** -100)
+    with np.errstate(all="ignore"):
+        s = np.where(zero, np.float32(1), a / m).astype(np.float32)
+        s[bad] = np.nan
+        z = v * (np.float32(1) / s)[:, None]
+    z[zero | bad] = 0
+    z = np.clip(z, -m, m)
+    q = np.zeros((x.shape[0], ld), np.float32)
+    q[:, :x.shape[1]] = np.rint(z) if t == "s8" else torch.from_numpy(z).to(F8).float().numpy()
+    return q, s
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("xt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols,ld,pad", [(1, 1, 1, 0), (1, 1, 16, 3), (3, 7, 7, 0), (5, 64, 64, 0), (2, 513, 520, 1),
+                                              (9, 1000, 1008, 0), (4, 2048, 2048, 8), (3, 4097, 4112, 0),
+                                              (2, 8192, 8192, 0), (3, 16384, 16384, 0), (2, 16391, 16400, 5),
+                                              (2, 40000, 40001, 0), (70, 300, 300, 4)])
+def test_quantize_rows_dyn(gpu, t, xt, rows, cols, ld, pad):
+    from dlq_amd import ops
+    rng = np.random.default_rng([rows, cols])
+    x = torch.from_numpy((rng.standard_normal((rows, cols)) * np.exp(2 * rng.standard_normal((rows, 1))))
+                         .astype(np.float32)).to(xt)
+    f = ops.quantize_rows_dyn_s8 if t == "s8" else ops.quantize_rows_dyn_f8
+    q, s = f(strided(x, pad, 1e30) if pad else x.cuda(), ld=ld)
+    rq, rs = quant_reference(x, t, ld)
+    assert np.array_equal(s.cpu().numpy(), rs)
+    got = q.cpu().float() if t == "s8" else q.cpu().view(F8).float()
+    assert np.array_equal(got.numpy(), rq)
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("cols", [20, 3000, 20000])
+def test_quantize_rows_dyn_edges(gpu, t, cols):
+    """Rows of zeros, subnormals, one infinity, one NaN, the largest floats."""
+    from dlq_amd import ops
+    x = torch.ones(9, cols)
+    x[0] = 0
+    x[1] = 1e-40
+    x[2, 7] = math.inf
+    x[3, cols - 1] = math.nan
+    x[4] = -3.4028234663852886e38
+    x[5] = 2.0 ** -100
+    x[6] = 2.0 ** -101
+    x[7, 0] = -math.inf
+    x[8] = torch.linspace(-5, 5, cols)
+    f = ops.quantize_rows_dyn_s8 if t == "s8" else ops.quantize_rows_dyn_f8
+    q, s = f(x.cuda())
+    rq, rs = quant_reference(x, t, cols)
+    assert np.array_equal(s.cpu().numpy(), rs, equal_nan=True)
+    got = q.cpu().float() if t == "s8" else q.cpu().view(F8).float()
+    assert np.array_equal(got.numpy(), rq)
+
+
+# -------------------------------------------------------- log probabilities
+
+def lp_bounds(x):
+    """64-bit log probabilities of finite-or-masked rows and the bounds of the
+    fp32 ones.  A term e^d of S is off by a factor of 1 + u (|d| + 4) (the
+    subtraction, the exponential), a sum of K terms over at least 64 lanes by
+    at most K/64 + 64 more additions; T's terms e^d d by one rounding more."""
+    x = x.double()
+    m = x.max(1, keepdim=True).values
+    d = torch.where(torch.isinf(m), x, x - m)
+    p = torch.softmax(d, 1).nan_to_num(0.0)
+    ls = torch.logsumexp(d, 1)
+    lp = torch.where(torch.isneginf(x), -math.inf, d - ls[:, None])
+    dz = torch.where(p > 0, d, 0.0)
+    n = x.shape[1] / 64 + 64
+    a1, a2 = (p * dz.abs()).sum(1), (p * dz * dz).sum(1)
+    ts = U * (n + 4 + a1)
+    lz = torch.where(torch.isinf(ls), 0.0, ls)
+    H = torch.where(torch.isinf(ls), 0.0, lz - (p * dz).sum(1))
+    tl = U * dz.abs().masked_fill(p <= 0, 0) + (ts + 2 * U * lz.abs())[:, None] + U * torch.nan_to_num(lp.abs(), posinf=0)
+    tl = tl + U * torch.where(torch.isneginf(d), 0.0, d.abs())
+    th = ts + U * (a2 + (n + 6) * a1) + a1 * ts + 4 * U * (lz.abs() + a1) + 1e-30
+    return lp, H, tl, th
+
+
+def alternatives(x, top):
+    """Descending values, equal ones by ascending index; NaN first."""
+    v = x.float().numpy().astype(np.float64)
+    v = np.where(np.isnan(v), np.inf, np.where(np.isposinf(v), 1e300, v))
+    return np.argsort(-v, axis=1, kind="stable")[:, :top].astype(np.int32)
+
+
+def check_logprobs(x, tokens, top, xdev=None):
+    from dlq_amd import ops
+    r = ops.logprobs(x.cuda() if xdev is None else xdev, None if tokens is None else tokens.cuda(), top)
+    lp, H, tl, th = lp_bounds(x.float())
+    close(r.entropy, H, th, "entropy")
+    if tokens is None:
+        assert r.logprob is None
+    else:
+        t = tokens.long()
+        at = t.clamp(min=0)[:, None]
+        want, tol = lp.gather(1, at)[:, 0], tl.gather(1, at)[:, 0]
+        got = r.logprob.cpu()
+        assert (got[t < 0] == 0).all()
+        inf = torch.isneginf(want) & (t >= 0)
+        assert torch.isneginf(got[inf]).all()
+        ok = ~inf & (t >= 0)
+        close(got[ok], want[ok], tol[ok], "logprob")
+    if top:
+        idx = alternatives(x, top)
+        assert np.array_equal(r.top_idx.cpu().numpy(), idx)
+        at = torch.from_numpy(idx).long()
+        want, got = lp.gather(1, at), r.top_logprob.cpu()
+        inf = torch.isneginf(want)
+        assert torch.isneginf(got[inf]).all()
+        close(got[~inf], want[~inf], tl.gather(1, at)[~inf], "top")
+    else:
+        assert r.top_idx is None
+    return r
+
+
+@pytest.mark.parametrize("xt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,K,top,pad", [(1, 1, 1, 0), (1, 1, 0, 0), (5, 2, 2, 0), (3, 8, 8, 1), (70, 64, 8, 0),
+                                            (9, 64, 64, 0), (7, 129, 20, 0), (4, 1000, 5, 0), (33, 1000, 64, 3),
+                                            (5, 2049, 20, 0), (3, 8192, 64, 0), (3, 8193, 64, 0), (2, 9001, 1, 7),
+                                            (2, 32003, 20, 0), (1, 100003, 64, 0), (6, 65536, 5, 0), (1, 300001, 0, 0)])
+def test_logprobs(gpu, xt, rows, K, top, pad):
+    rng = np.random.default_rng([rows, K])
+    x = torch.from_numpy((rng.standard_normal((rows, K)) * 3).astype(np.float32)).to(xt)  # bf16: many ties
+    tokens = torch.from_numpy(rng.integers(-1, K, rows).astype(np.int32))
+    check_logprobs(x, tokens, top, strided(x, pad, math.nan) if pad else None)
+
+
+@pytest.mark.parametrize("K,top", [(50, 50), (3000, 64), (20000, 64), (70000, 20)])
+def test_logprobs_masked_and_tied(gpu, K, top):
+    rng = np.random.default_rng(K)
+    x = torch.from_numpy(rng.standard_normal((12, K)).astype(np.float32))
+    x[0] = -math.inf                       # nothing left
+    x[1] = -math.inf
+    x[1, K // 2] = 2.0                     # one left
+    x[2] = 0.0                             # all equal
+    x[3] = torch.arange(K) * 1e-3          # ascending
+    x[4] = -torch.arange(K) * 1e-3         # descending
+    x[5] = torch.finfo(torch.float32).min  # masked with the lowest value
+    x[6] = torch.finfo(torch.float32).min
+    x[6, 3] = 1.0
+    x[7, ::2] = -math.inf
+    x[8] = torch.where(torch.arange(K) % 2 == 0, 0.0, -0.0)  # zeros of both signs are equal
+    x[9, -1] = 200.0
+    x[10] = x[10] * 1e30
+    x[11, : K - 3] = -math.inf
+    tokens = torch.tensor([0, K // 2, 5, K - 1, 0, 1, 3, 1, 2, K - 1, 0, K - 1], dtype=torch.int32)
+    r = check_logprobs(x, tokens, top)
+    assert r.entropy[0] == 0 and r.entropy[1] == 0 and torch.isneginf(r.logprob[0])
+
+
+@pytest.mark.parametrize("K", [40, 5000, 30000])
+def test_logprobs_not_finite(gpu, K):
+    """NaN and +inf make their row's numbers NaN, the order stays defined."""
+    from dlq_amd import ops
+    rng = np.random.default_rng(1)
+    x = torch.from_numpy(rng.standard_normal((5, K)).astype(np.float32))
+    x[0, 0] = math.nan
+    x[1, K - 1] = math.nan
+    x[2, 7] = math.inf
+    x[3, 5], x[3, 9], x[3, 11] = math.inf, math.nan, math.inf
+    r = ops.logprobs(x.cuda(), torch.tensor([1, 2, 3, 4, K], dtype=torch.int32, device="cuda"), 6)
+    assert r.logprob.isnan().all()  # the last row's token lies outside
+    assert r.entropy[:4].isnan().all() and r.top_logprob[:4].isnan().all()
+    assert torch.isfinite(r.entropy[4]) and torch.isfinite(r.top_logprob[4]).all()
+    assert np.array_equal(r.top_idx.cpu().numpy(), alternatives(x, 6))
+
+
+def test_logprobs_offsets_past_32_bits(gpu):
+    rng = np.random.default_rng(6)
+    rows, K, ld = 3, 9000, 1_200_000_000
+    x = torch.from_numpy(rng.standard_normal((rows, K)).astype(np.float32)).to(torch.bfloat16)
+    big = torch.empty(2 * ld + K, dtype=torch.bfloat16, device="cuda")
+    v = big.as_strided((rows, K), (ld, 1))
+    v.copy_(x)
+    check_logprobs(x, torch.tensor([1, 2, 3], dtype=torch.int32), 4, v)
+    del big, v
+    torch.cuda.empty_cache()
+
+
+# ------------------------------------------------- together, streams, graphs
+
+def make_layer(seed, t, d, h, E, V):
+    """Weights of a routed layer and its head, quantised per output channel."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def weights(*shape):
+        w = torch.randn(*shape, generator=g, device="cuda") / shape[-1] ** 0.5
+        m = 127.0 if t == "s8" else 448.0
+        s = w.abs().amax(-1) / m
+        v = w / s[..., None]
+        return (v.round().to(torch.int8) if t == "s8" else v.to(F8).view(torch.uint8)), s
+
+    return dict(router=weights(E, d), up=weights(E, h, d), down=weights(E, d, h), head=weights(V, d),
+                b=torch.randn(E, h, generator=g, device="cuda") * 0.1)
+
+
+def routed_layer(L, hidden, t, tokens, top):
+    """hidden [T, d] bf16 -> the answer's log probabilities: every step of the
+    product is one of the row operators, the routing between is torch's."""
+    from dlq_amd import ops
+    dense, grouped = linear(t)
+    quant = ops.quantize_rows_dyn_s8 if t == "s8" else ops.quantize_rows_dyn_f8
+    T, E = hidden.shape[0], L["up"][0].shape[0]
+    q, s = quant(hidden)
+    r = ops.logprobs(dense(q, L["router"][0], s, L["router"][1]), None, 2)
+    p = r.top_logprob.exp()
+    order = r.top_idx.reshape(-1).argsort(stable=True)
+    rows = order // 2
+    off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    off[1:] = torch.bincount(r.top_idx.reshape(-1), minlength=E).cumsum(0)
+    u = grouped(q[rows], off, L["up"][0], s[rows], L["up"][1], L["b"], "silu", out_dtype=torch.bfloat16)
+    uq, us = quant(u)
+    o = grouped(uq, off, L["down"][0], us, L["down"][1], out_dtype=torch.float32)
+    hidden = hidden.float().index_add(0, rows, o * p.reshape(-1)[order, None]).to(torch.bfloat16)
+    q, s = quant(hidden)
+    logits = dense(q, L["head"][0], s, L["head"][1], out_dtype=torch.float32)
+    return r, hidden, logits, ops.logprobs(logits, tokens, top)
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("T", [1, 37])
+def test_routed_layer_together(gpu, t, T):
+    """The operators as a decoder layer uses them, against the same layer in
+    64 bits on the codes and choices that came out (each operator is bounded
+    by its own tests; here the parts have to fit together)."""
+    d, h, E, V = 256, 320, 8, 2000
+    L = make_layer(1, t, d, h, E, V)
+    hidden = torch.randn(T, d, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").bfloat16()
+    tokens = torch.arange(T, dtype=torch.int32, device="cuda") * 7 % V
+    r, out, logits, ans = routed_layer(L, hidden, t, tokens, 5)
+    w = {k: values(L[k][0]) * L[k][1].double()[..., None] for k in ("router", "up", "down", "head")}
+    x = hidden.double()
+    # int8 rows are off by half of max|x|/127 per value, e4m3 codes by 2^-4 of the value, each
+    # independent: over d terms of a unit-norm weight row that is a few percent of the row's size
+    ref = x.clone()
+    for k in range(2):
+        e = r.top_idx[:, k].long()
+        u = torch.einsum("thd,td->th", w["up"][e], x) + L["b"].double()[e]
+        ref += r.top_logprob[:, k].double().exp()[:, None] * torch.einsum("tdh,th->td", w["down"][e], act64(u, "silu"))
+    err = float((out.double() - ref).norm() / ref.norm())
+    assert err < 0.03, err
+    lg = out.double() @ w["head"].T
+    assert float((logits.double() - lg).norm() / lg.norm()) < 0.06
+    lp, H, tl, th = lp_bounds(logits.cpu())
+    close(ans.entropy, H, th)
+    close(ans.logprob, lp.gather(1, tokens.cpu().long()[:, None])[:, 0], tl.gather(1, tokens.cpu().long()[:, None])[:, 0])
+    assert np.array_equal(ans.top_idx.cpu().numpy(), alternatives(logits.cpu(), 5))
+
+
+def flat(res):
+    r, hidden, logits, ans = res
+    return [r.top_idx, r.top_logprob, r.entropy, hidden, logits, *ans]
+
+
+def test_rowops_repeat_and_other_stream(gpu):
+    """The same bits on every run and on another stream."""
+    L = make_layer(3, "s8", 256, 320, 8, 9000)
+    hidden = torch.randn(50, 256, device="cuda").bfloat16()
+    tokens = torch.arange(50, dtype=torch.int32, device="cuda")
+
+    def ops_only():  # no library sums between (index_add may reorder them)
+        from dlq_amd import ops
+        q, s = ops.quantize_rows_dyn_s8(hidden)
+        y = ops.linear_act_s8(q, L["head"][0], s, L["head"][1], out_dtype=torch.bfloat16)
+        return [q, s, y, *ops.logprobs(y, tokens, 20)]
+
+    a = ops_only()
+    b = ops_only()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c = ops_only()
+    torch.cuda.current_stream().wait_stream(side)
+    for u, v, w in zip(a, b, c):
+        assert torch.equal(u, v) and torch.equal(u, w)
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+def test_rowops_graph(gpu, t):
+    """Two captured graphs with eager work between their replays, each replay
+    against the eager result."""
+    from dlq_amd import ops
+    dense, grouped = linear(t)
+    quant = ops.quantize_rows_dyn_s8 if t == "s8" else ops.quantize_rows_dyn_f8
+    L = make_layer(4, t, 256, 320, 8, 30000)
+    off = torch.tensor([0, 9, 9, 20, 21, 30, 33, 40, 44], dtype=torch.int32, device="cuda")
+    tokens = torch.arange(48, dtype=torch.int32, device="cuda")
+
+    def step(x, res, y):
+        q, s = quant(x)
+        u = grouped(q, off, L["up"][0], s, L["up"][1], L["b"], "gelu", out=y)
+        uq, us = quant(u)
+        v = grouped(uq, off, L["down"][0], us, L["down"][1], residual=res, out=res.clone())
+        vq, vs = quant(v)
+        logits = dense(vq, L["head"][0], vs, L["head"][1])
+        return [v, logits, *ops.logprobs(logits, tokens, 20)]
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    xs = [torch.randn(48, 256, generator=gen, device="cuda").bfloat16() for _ in range(2)]
+    res = torch.randn(48, 256, generator=gen, device="cuda")
+    ys = [torch.zeros(48, 320, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for x, y in zip(xs, ys):
+            step(x, res, y)
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y in zip(xs, ys):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(x, res, y))
+        graphs.append(g)
+    for rep in range(4):
+        for k in (0, 1) if rep % 2 else (1, 0):
+            xs[k].copy_(torch.randn(48, 256, generator=gen, device="cuda"))
+            graphs[k].replay()
+        for k in (0, 1):
+            want = step(xs[k], res, torch.zeros_like(ys[k]))
+            torch.cuda.synchronize()
+            for a, b in zip(outs[k], want):
+                assert torch.equal(a, b), (rep, k)
+
+
+def test_ops_check_devices_and_shapes(gpu):
+    from dlq_amd import ops
+    x = torch.zeros(4, 32, dtype=torch.int8, device="cuda")
+    w = torch.zeros(8, 32, dtype=torch.int8, device="cuda")
+    s = torch.ones(8, device="cuda")
+    with pytest.raises(ValueError):
+        ops.linear_act_s8(x, w[:, :16], None, s)
+    with pytest.raises(ValueError):
+        ops.linear_act_s8(x, w, torch.ones(3, device="cuda"), s)
+    with pytest.raises(ValueError):
+        ops.linear_act_s8(x, w, None, s, out=torch.zeros(4, 9, device="cuda"))
+    with pytest.raises(TypeError):
+        ops.linear_act_s8(x, w, None, s, residual=torch.zeros(4, 8, device="cuda"), out_dtype=torch.bfloat16)
+    with pytest.raises(TypeError):
+        ops.linear_act_s8(x, w, None, None)
+    with pytest.raises(ValueError):
+        ops.linear_act_s8(x.T, w.T, None, s)
+    with pytest.raises(ValueError):
+        ops.linear_act_s8(x[:1].expand(4, 32), w, None, s)
+    with pytest.raises(ValueError):
+        ops.linear_grouped_s8(x, torch.zeros(3, dtype=torch.int32, device="cuda"), w[None], None, s[None])
+    with pytest.raises(TypeError):
+        ops.linear_grouped_s8(x, torch.zeros(2, dtype=torch.int64, device="cuda"), w[None], None, s[None])
+    with pytest.raises(RuntimeError):
+        ops.logprobs(torch.zeros(2, 8, device="cuda"), None, 9)
+    with pytest.raises(TypeError):
+        ops.logprobs(torch.zeros(2, 8, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda"))
+    assert ops.linear_act_s8(x[:0], w, None, s).shape == (0, 8)
+    assert ops.logprobs(torch.zeros(0, 8, device="cuda"), top=2).top_idx.shape == (0, 2)
+    assert ops.quantize_rows_dyn_s8(torch.zeros(0, 8, device="cuda"))[0].shape == (0, 8)
