@@ -28,53 +28,94 @@ struct LinearArgs {
   const int* off;      // [E + 1], E > 0
 };
 
-__device__ __forceinline__ float act_of(float v, int act) {
+// The activations on the hardware's exp2 and reciprocal (1 ulp each).
+//  * GELU's erf by Abramowitz and Stegun 7.1.26, off by at most 1.5e-7:
+//    erf(z) = 1 - (a1 t + .. + a5 t^5) e^(-z^2), t = 1 / (1 + p z), z >= 0;
+//    v/2 (1 + erf(v / sqrt 2)) = max(v, 0) - |v|/2 poly e^(-v^2/2).
+//  * GELU_TANH: 1 + tanh(u) = 2 / (1 + e^-2u).
+template <int ACT>
+__device__ __forceinline__ float act_of(float v) {
+  if constexpr (ACT == DLQ_ACT_RELU) return v < 0.f ? 0.f : v;  // a NaN stays
+  if constexpr (ACT == DLQ_ACT_GELU) {
+    // y = z sqrt(log2 e): e^(-z^2) = 2^(-y^2); y stays finite so that y * 0 is 0 for an infinite v
+    const float y = __builtin_fminf(__builtin_fabsf(v) * 0.84932180028801905f, 1e15f);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.27273743f, y, 1.f));  // p / sqrt(log2 e)
+    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    p = __builtin_fmaf(p, t, 1.421413741f);
+    p = __builtin_fmaf(p, t, -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.254829592f) * t;
+    // |v|/2 = y / (2 * 0.8493..)
+    return __builtin_fmaf(y * p, -0.58870501f * __builtin_amdgcn_exp2f(-y * y), v < 0.f ? 0.f : v);
+  }
+  if constexpr (ACT == DLQ_ACT_GELU_TANH) {
+    const float u = v * __builtin_fmaf(0.044715f * v, v, 1.f) * (1.5957691216057308f * 1.4426950408889634f);
+    return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-u));
+  }
+  if constexpr (ACT == DLQ_ACT_SILU)
+    return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+  return v;
+}
+
+// f(constant of the activation): one branch around a loop, not one per value
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F f) {
   switch (act) {
-    case DLQ_ACT_RELU: return v < 0.f ? 0.f : v;  // a NaN stays
-    case DLQ_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-    case DLQ_ACT_GELU_TANH: {  // 1 + tanh(u) = 2 / (1 + e^-2u)
-      const float u = v * __builtin_fmaf(0.044715f * v, v, 1.f) * 1.5957691216057308f;
-      return v / (1.f + expf(-u));
-    }
-    case DLQ_ACT_SILU: return v / (1.f + expf(-v));
-    default: return v;
+    case DLQ_ACT_RELU: f(std::integral_constant<int, DLQ_ACT_RELU>{}); break;
+    case DLQ_ACT_GELU: f(std::integral_constant<int, DLQ_ACT_GELU>{}); break;
+    case DLQ_ACT_GELU_TANH: f(std::integral_constant<int, DLQ_ACT_GELU_TANH>{}); break;
+    case DLQ_ACT_SILU: f(std::integral_constant<int, DLQ_ACT_SILU>{}); break;
+    default: f(std::integral_constant<int, DLQ_ACT_NONE>{}); break;
   }
 }
 
-// Four accumulators of row m, columns n..n+3 of expert e (0 if not grouped).
-__device__ __forceinline__ void store4(const LinearArgs& a, int e, int m, int n, const float* acc) {
-  const float sx = a.xs ? a.xs[m] : 1.f;
-  const size_t en = (size_t)e * a.N + n, ym = (size_t)m * a.ldy + n, rm = (size_t)m * a.ldr + n;
-  if (a.vec && n + 4 <= a.N) {
-    const v4f ws = *(const v4f*)(a.ws + en);
-    v4f b = {0.f, 0.f, 0.f, 0.f}, v;
-    if (a.bias) b = *(const v4f*)(a.bias + en);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = act_of(__builtin_fmaf(acc[i], sx * ws[i], b[i]), a.act);
-    if (a.bf16) {
-      if (a.res) {
-        const v2u r = *(const v2u*)((const uint16_t*)a.res + rm);
-        v += v4f{bf_lo(r[0]), bf_hi(r[0]), bf_lo(r[1]), bf_hi(r[1])};
-      }
-      *(v2u*)((uint16_t*)a.y + ym) = v2u{bf_pack(v[0], v[1]), bf_pack(v[2], v[3])};
-    } else {
-      if (a.res) v += *(const v4f*)((const float*)a.res + rm);
-      *(v4f*)((float*)a.y + ym) = v;
-    }
-    return;
-  }
+// The residual's / the output's columns n..n+3 of row m, all of them below N
+// and aligned (a.vec).
+__device__ __forceinline__ v4f residual4(const LinearArgs& a, int m, int n) {
+  const size_t at = (size_t)m * a.ldr + n;
+  if (!a.bf16) return *(const v4f*)((const float*)a.res + at);
+  const v2u r = *(const v2u*)((const uint16_t*)a.res + at);
+  return v4f{bf_lo(r[0]), bf_hi(r[0]), bf_lo(r[1]), bf_hi(r[1])};
+}
+__device__ __forceinline__ void put4(const LinearArgs& a, int m, int n, v4f v) {
+  const size_t at = (size_t)m * a.ldy + n;
+  if (a.bf16)
+    *(v2u*)((uint16_t*)a.y + at) = v2u{bf_pack(v[0], v[1]), bf_pack(v[2], v[3])};
+  else
+    *(v4f*)((float*)a.y + at) = v;
+}
+// The same, residual and output, one column at a time and those past N left out.
+__device__ __forceinline__ void put4_any(const LinearArgs& a, int m, int n, v4f v) {
+  const size_t ym = (size_t)m * a.ldy + n, rm = (size_t)m * a.ldr + n;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (n + i >= a.N) break;
-    float v = act_of(__builtin_fmaf(acc[i], sx * a.ws[en + i], a.bias ? a.bias[en + i] : 0.f), a.act);
     if (a.bf16) {
-      if (a.res) v += __uint_as_float((unsigned)((const uint16_t*)a.res)[rm + i] << 16);
-      ((uint16_t*)a.y)[ym + i] = (uint16_t)bf_pack(v, 0.f);
+      if (a.res) v[i] += __uint_as_float((unsigned)((const uint16_t*)a.res)[rm + i] << 16);
+      ((uint16_t*)a.y)[ym + i] = (uint16_t)bf_pack(v[i], 0.f);
     } else {
-      if (a.res) v += ((const float*)a.res)[rm + i];
-      ((float*)a.y)[ym + i] = v;
+      if (a.res) v[i] += ((const float*)a.res)[rm + i];
+      ((float*)a.y)[ym + i] = v[i];
     }
   }
+}
+// act(fma(acc, sx ws, b)) of four columns
+template <int ACT>
+__device__ __forceinline__ v4f scaled4(v4f acc, float sx, v4f ws, v4f b) {
+  v4f v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = act_of<ACT>(__builtin_fmaf(acc[i], sx * ws[i], b[i]));
+  return v;
+}
+
+// p[n..n+3] of N values; those past N (and all of a null p) are 0.
+__device__ __forceinline__ v4f column4(const float* p, int n, int N, int vec) {
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+  if (!p) return v;
+  if (vec) return *(const v4f*)(p + n);  // N % 4 == 0
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < N) v[i] = p[n + i];
+  return v;
 }
 
 // The t-th tile of BM rows over all experts: its expert e and rows [m0, m1);
@@ -162,15 +203,17 @@ struct Mma<true> {
 // workgroup, its WK waves each take a slice of K and join their sums in LDS
 // (in wave order).  Lane l holds row l & 15, 16 bytes at 16 (l >> 4) of every
 // 64: the order of K within a step is free as long as both operands agree.
-template <bool F8, int MI, int NJ, int WK>
-__global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs a) {
+template <bool F8, int MI, int NJ, int WK, int U>
+__global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs a, int nbm) {
   typedef Mma<F8> MM;
   typedef typename MM::acc_t acc_t;
   constexpr int BM = 16 * MI, BN = 16 * NJ, KB = 64;
   __shared__ acc_t part[WK][MI * NJ][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
-  const int nbn = (a.N + BN - 1) / BN;
-  const int n0 = (int)(blockIdx.x % nbn) * BN, mt = blockIdx.x / nbn;
+  // each XCD takes a run of tiles, row tiles fastest: those that share weights
+  // run side by side on one L2
+  const int l = xcd_remap(blockIdx.x, gridDim.x);
+  const int n0 = l / nbm * BN, mt = l % nbm;
   int e = 0, m0 = mt * BM, m1 = a.M;
   if (a.E && !expert_tile<BM>(a, mt, e, m0, m1)) return;
 
@@ -193,29 +236,56 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
 
   const int steps = (a.K + KB - 1) / KB, full = a.K / KB;
   const int s0 = (int)((long)steps * wave / WK), s1 = (int)((long)steps * (wave + 1) / WK);
-  for (int s = s0; s < s1; ++s) {
-    v4i rx[MI], rw[NJ];
-    if (s < full) {
+  // U steps' loads are on their way while U others are multiplied
+  v4i rx[2][U][MI], rw[2][U][NJ];
+  auto load = [&](int b, int s) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) rx[i] = *(const v4i_any*)(xp[i] + (size_t)s * KB);
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) rw[j] = *(const v4i_any*)(wp[j] + (size_t)s * KB);
-    } else {  // the end of K: zeros past it
-      const int k = s * KB, avail = a.K - k - 16 * lg;
+      for (int j = 0; j < NJ; ++j) rw[b][u][j] = *(const v4i_any*)(wp[j] + (size_t)(s + u) * KB);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) rx[i] = load_codes16(xp[i] + k, avail);
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) rw[j] = load_codes16(wp[j] + k, avail);
+      for (int i = 0; i < MI; ++i) rx[b][u][i] = *(const v4i_any*)(xp[i] + (size_t)(s + u) * KB);
     }
-    typename MM::frag fx[MI], fw[NJ];
+  };
+  auto multiply = [&](int b, int n) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i) fx[i] = MM::prep(rx[i]);
+    for (int u = 0; u < n; ++u) {
+      typename MM::frag fx[MI], fw[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) fw[j] = MM::prep(rw[j]);
+      for (int i = 0; i < MI; ++i) fx[i] = MM::prep(rx[b][u][i]);
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+      for (int j = 0; j < NJ; ++j) fw[j] = MM::prep(rw[b][u][j]);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[i][j] = MM::go(fw[j], fx[i], acc[i][j]);
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = MM::go(fw[j], fx[i], acc[i][j]);
+    }
+  };
+  const int sf = s1 < full ? s1 : full;
+  int s = s0;
+  if (s + U <= sf) load(0, s);
+  for (; s + 3 * U <= sf; s += 2 * U) {
+    load(1, s + U);
+    multiply(0, U);
+    load(0, s + 2 * U);
+    multiply(1, U);
+  }
+  if (s + 2 * U <= sf) {
+    load(1, s + U);
+    multiply(0, U);
+    multiply(1, U);
+    s += 2 * U;
+  } else if (s + U <= sf) {
+    multiply(0, U);
+    s += U;
+  }
+  for (; s < s1; ++s) {
+    const int k = s * KB, avail = s < full ? 16 : a.K - k - 16 * lg;  // the end of K: zeros past it
+#pragma unroll
+    for (int i = 0; i < MI; ++i) rx[0][0][i] = load_codes16(xp[i] + k, avail);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) rw[0][0][j] = load_codes16(wp[j] + k, avail);
+    multiply(0, 1);
   }
 #pragma unroll
   for (int i = 0; i < MI; ++i)
@@ -227,43 +297,444 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
 #pragma unroll
     for (int k = 1; k < WK; ++k) s += part[k][t][lane];
     const int m = m0 + 16 * (t / NJ) + lr, n = n0 + 16 * (t % NJ) + 4 * lg;
-    const float v[4] = {(float)s[0], (float)s[1], (float)s[2], (float)s[3]};
-    if (m < m1) store4(a, e, m, n, v);
+    if (m < m1 && n < a.N) {
+      const float sx = a.xs ? a.xs[m] : 1.f;
+      const v4f ws = column4(a.ws + (size_t)e * a.N, n, a.N, a.vec);
+      const v4f b = column4(a.bias ? a.bias + (size_t)e * a.N : nullptr, n, a.N, a.vec);
+      v4f v, r = {0.f, 0.f, 0.f, 0.f};
+      if (a.vec && a.res) r = residual4(a, m, n);
+      with_act(a.act, [&](auto act) {
+        v = scaled4<decltype(act)::value>(v4f{(float)s[0], (float)s[1], (float)s[2], (float)s[3]}, sx, ws, b);
+      });
+      if (!a.vec)
+        put4_any(a, m, n, v);
+      else
+        put4(a, m, n, a.res ? v + r : v);
+    }
   }
 }
 
-template <bool F8, int MI, int NJ, int WK>
+// ---- large products: tiles through LDS ------------------------------------
+// TN columns (rows of w) by TM rows of x per workgroup of WN x WM waves, each
+// wave NI x MJ tiles of 32 x 32.  Both operands stream by LDS-DMA, 128 bytes
+// of K per stage into two slots; row r of a slot is 128 bytes, its 16-byte
+// chunk c at 16 (c ^ ((r >> 1) & 7)), so the 16 rows a ds_read_b128 lane group
+// reads fall on 16 distinct bank quads (the DMA lanes fetch in that order).
+//
+// The pipeline of a wave: while the matrix instructions of one K step run, the
+// fragments of the next are read.  Before the last step of a stage one barrier
+// says both that the next stage has landed everywhere and that nobody reads
+// this stage's slot any more; behind it the next stage's first fragments are
+// read and the DMA of the stage after the next is issued, one piece behind
+// each matrix instruction.  So a stage has all but one of a stage's steps to
+// land, and no matrix instruction waits for a fragment read issued right
+// before it.
+//
+// Waves own 128 x 128 outputs where there are enough rows and columns: an LDS
+// byte then feeds 64 multiply-adds, and reads and DMA writes take 192 KB of
+// the 256 KB that LDS moves in a stage's 2048 matrix cycles (with 128 x 64
+// per wave: 256 KB, the bound).
+//
+// e4m3 here uses the fp8 matrix instructions, whose cut products (see Mma) are
+// off by up to 7 * 2^-13 of the largest of each 8: 1.4e-5 of the result on
+// normal data, which bf16's rounding (2^-9) hides; only bf16 outputs come here.
+template <bool F8>
+struct TileMma {
+  typedef v16i acc_t;
+  typedef v4i sum4;
+  static constexpr int NV = 1;  // 16-byte reads per fragment
+  static __device__ __forceinline__ v16i go(const v4i* a, const v4i* b, v16i c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a[0], b[0], c, 0, 0, 0);
+  }
+};
+template <>
+struct TileMma<true> {
+  typedef v16f acc_t;
+  typedef v4f sum4;
+  static constexpr int NV = 2;
+  static __device__ __forceinline__ v16f go(const v4i* a, const v4i* b, v16f c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat8(a[0], a[1]), cat8(b[0], b[1]), c, 0, 0, 0, 0, 0, 0);
+  }
+};
+
+__device__ __attribute__((aligned(64))) int8_t g_zero_linear[64];
+
+// a pointer that is the same in every lane, told to the compiler
+__device__ __forceinline__ const int8_t* uniform(const int8_t* p) {
+  const unsigned long long v = (unsigned long long)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+  return (const int8_t*)((unsigned long long)hi << 32 | lo);
+}
+
+template <bool F8, int WN, int WM, int NI, int MJ, int KB, int SLOTS, int WPE>
+__global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const LinearArgs a, int nbm, int nbn) {
+  typedef TileMma<F8> MM;
+  typedef typename MM::acc_t acc_t;
+  typedef typename MM::sum4 sum4;
+  constexpr int NW = WN * WM, TN = 32 * WN * NI, TM = 32 * WM * MJ, NV = MM::NV;
+  constexpr int SPS = KB / 32 / NV;                        // K steps of a stage
+  constexpr int CPR = KB / 16, RPP = 64 / CPR;             // chunks of a row, rows of a 1 KiB piece
+  constexpr int SLOT = (TN + TM) * KB;
+  constexpr int PW = TN / RPP / NW, PX = TM / RPP / NW, PP = PW + PX;  // pieces of a stage per wave
+  constexpr int NM = NI * MJ, NR = (NI + MJ) * NV;
+  static_assert(KB == 128 || KB == 64, "chunk swizzle");
+  static_assert(NW % 2 == 0 && TN % (RPP * NW) == 0 && TM % (RPP * NW) == 0, "pieces per wave");
+  static_assert(PP * (SLOTS - 1) <= 63, "counted waits");
+  constexpr int PITCH = NI * 32 * 4 + 16;  // epilogue staging: 32 rows of a wave's columns
+  static_assert(NW * 32 * PITCH <= SLOTS * SLOT, "epilogue staging");
+  __shared__ __attribute__((aligned(16))) int8_t lds[SLOTS * SLOT];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 31, lh = lane >> 5, wn = wave % WN, wm = wave / WN;
+  // each XCD takes a run of tiles, down groups of 4 row blocks column by column
+  constexpr int GROW = 4;
+  const int l = xcd_remap(blockIdx.x, gridDim.x);
+  const int grp = l / (GROW * nbn), r0 = grp * GROW;
+  const int gsz = nbm - r0 < GROW ? nbm - r0 : GROW, li = l - grp * GROW * nbn;
+  const int mt = r0 + li % gsz, n0 = li / gsz * TN;
+  int e = 0, m0 = mt * TM, m1 = a.M;
+  if (a.E) {
+    if (!expert_tile<TM>(a, mt, e, m0, m1)) return;
+    e = __builtin_amdgcn_readfirstlane(e);
+    m0 = __builtin_amdgcn_readfirstlane(m0);
+    m1 = __builtin_amdgcn_readfirstlane(m1);
+  }
+  const int8_t* wbase = uniform(a.w + ((size_t)e * a.N + n0) * a.ldw);
+  const int8_t* xbase = uniform(a.x + (size_t)m0 * a.ldx);
+
+  // piece r of this wave: rows RPP (wave + NW r) ..; rows past the end repeat
+  // the last one (they are not stored).  The swizzle is the same for all r.
+  const auto swizzle = [](int row) { return KB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
+  const int prow = RPP * wave + lane / CPR, chunk = (lane % CPR) ^ swizzle(prow);
+  unsigned vw[PW], vx[PX];
+#pragma unroll
+  for (int r = 0; r < PW; ++r) {
+    const int n = prow + RPP * NW * r, last = a.N - 1 - n0;
+    vw[r] = (unsigned)(n < last ? n : last) * (unsigned)a.ldw + 16 * chunk;
+  }
+#pragma unroll
+  for (int r = 0; r < PX; ++r) {
+    const int m = prow + RPP * NW * r, last = m1 - 1 - m0;
+    vx[r] = (unsigned)(m < last ? m : last) * (unsigned)a.ldx + 16 * chunk;
+  }
+  const unsigned lds32 = lds_addr32(lds);
+  const int nst = (a.K + KB - 1) / KB, full = a.K / KB;
+  const int8_t* zsrc = g_zero_linear;
+  asm volatile("" : "+s"(zsrc));
+  // piece r of stage st into a slot; whole: all of the stage lies within K
+  auto issue = [&](int st, int slot, int r, bool whole) __attribute__((always_inline)) {
+    const unsigned to = lds32 + slot * SLOT + (r < PW ? 0 : TN * KB) + (wave + NW * (r < PW ? r : r - PW)) * 1024;
+    const int8_t* base = (r < PW ? wbase : xbase) + (size_t)st * KB;
+    const unsigned v = r < PW ? vw[r < PW ? r : 0] : vx[r < PW ? 0 : r - PW];
+    if (whole || st < full)
+      glds16_saddr(base, v, to);
+    else if (st < nst)  // the end of K: zeros past it
+      glds16_asm(st * KB + 16 * chunk < a.K ? base + v : zsrc, to);
+  };
+
+  acc_t acc[NI][MJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) acc[i][j] = acc_t{0};
+  v4i fw[2][NI][NV], fx[2][MJ][NV];
+  const int sw = swizzle(lr);
+  // read q of step `step` of a slot into buffer b (in the order of first use)
+  auto read = [&](int slot, int step, int b, int q) __attribute__((always_inline)) {
+    const int v = q % NV, f = q / NV, c = (step * NV + v) * 2 + lh;
+    const int8_t* p = lds + slot * SLOT + 16 * (c ^ sw);
+    if (f == 0)
+      fw[b][0][v] = *(const v4i*)(p + (wn * NI * 32 + lr) * KB);
+    else if (f <= MJ)
+      fx[b][f - 1][v] = *(const v4i*)(p + TN * KB + ((wm * MJ + f - 1) * 32 + lr) * KB);
+    else
+      fw[b][f - MJ][v] = *(const v4i*)(p + ((wn * NI + f - MJ) * 32 + lr) * KB);
+  };
+  // one step's matrix instructions on buffer b; behind instruction t come reads
+  // of the next step (rslot >= 0) and DMA pieces of stage dst (dst >= 0)
+  auto step = [&](int b, int rslot, int rstep, int dst, int dslot, bool whole) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < NM; ++t) {
+      const int i = t / MJ, j = t % MJ;
+      acc[i][j] = MM::go(fw[b][i], fx[b][j], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (rslot >= 0) {
+#pragma unroll
+        for (int q = 0; q < NR; ++q)
+          if (q * NM / NR == t) read(rslot, rstep, b ^ 1, q);
+      }
+      if (dst >= 0) {
+#pragma unroll
+        for (int r = 0; r < PP; ++r)
+          if (r * NM / PP == t) issue(dst, dslot, r, whole);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // stage s, its first fragments in buffer b0; slot: where it lies, next: the
+  // slot of s + 1.  Before its last step: stage s + 1 has landed everywhere,
+  // and nobody reads stage s's slot any more, which stage s + SLOTS then takes.
+  auto stage = [&](int s, int slot, int next, int b0, bool whole) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k + 1 < SPS; ++k) step((b0 + k) & 1, slot, k + 1, -1, 0, false);
+    if (whole) {
+      wait_vm_const<PP*(SLOTS - 2)>();  // and lgkmcnt(0)
+    } else {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    }
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    step((b0 + SPS - 1) & 1, next, 0, s + SLOTS, slot, whole);
+  };
+
+#pragma unroll
+  for (int st = 0; st < SLOTS; ++st)
+#pragma unroll
+    for (int r = 0; r < PP; ++r) issue(st, st, r, false);
+  // the epilogue's operands, on their way before the sums begin
+  constexpr int LPR = NI * 8, RPI = 64 / LPR, U = 4;  // lanes per row, rows per instruction, instructions in flight
+  static_assert(32 % (RPI * U) == 0, "rows of a staging pass");
+  const int cn = n0 + wn * NI * 32 + 4 * (lane % LPR), cr = lane / LPR;
+  const bool in = cn < a.N;
+  v4f ws = {0.f, 0.f, 0.f, 0.f}, bias = ws;
+  if (in) {
+    ws = column4(a.ws + (size_t)e * a.N, cn, a.N, a.vec);
+    bias = column4(a.bias ? a.bias + (size_t)e * a.N : nullptr, cn, a.N, a.vec);
+  }
+  float sxr[MJ];
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    const int m = m0 + (wm * MJ + j) * 32 + lr;
+    sxr[j] = a.xs && m < m1 ? a.xs[m] : 1.f;
+  }
+  if (nst >= SLOTS)
+    wait_vm_const<PP*(SLOTS - 1)>();  // stage 0 has landed, the others may be under way
+  else
+    wait_vm0();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if (nst > 0) {
+#pragma unroll
+    for (int q = 0; q < NR; ++q) read(0, 0, 0, q);
+    int s = 0, slot = 0;
+    const auto after = [](int k) { return k + 1 == SLOTS ? 0 : k + 1; };
+    // two stages at a time where a stage is an odd number of steps: the
+    // fragment buffers are then compile-time
+    constexpr int AT = SPS & 1 ? 2 : 1;
+    for (; s + AT - 1 + SLOTS < full; s += AT) {
+#pragma unroll
+      for (int u = 0; u < AT; ++u) {
+        stage(s + u, slot, after(slot), u * SPS & 1, true);
+        slot = after(slot);
+      }
+    }
+    for (; s + AT < nst; s += AT) {
+#pragma unroll
+      for (int u = 0; u < AT; ++u) {
+        stage(s + u, slot, after(slot), u * SPS & 1, false);
+        slot = after(slot);
+      }
+    }
+    if (AT == 2 && s + 1 < nst) {
+      stage(s, slot, after(slot), 0, false);
+      slot = after(slot);
+      step(1, -1, 0, -1, 0, false);
+    } else {
+#pragma unroll
+      for (int k = 0; k + 1 < SPS; ++k) step(k & 1, slot, k + 1, -1, 0, false);
+      step((SPS - 1) & 1, -1, 0, -1, 0, false);
+    }
+  }
+  __syncthreads();  // the slots become the epilogue's staging
+
+  // Through LDS, a wave's 32 rows at a time, into rows: lane t then holds four
+  // consecutive columns of one row, whole cache lines of y per instruction.
+  // The row's scale rides in the pitch's padding.  The loop over the row code
+  // is a real one (only the accumulator reads are per j): unrolled, with five
+  // activations, the epilogue outgrew the instruction cache and cost as much
+  // as 4096 of K.
+  int8_t* mine = lds + wave * 32 * PITCH;
+  auto stage_out = [&](auto jc) __attribute__((always_inline)) {
+    constexpr int j = decltype(jc)::value;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)  // accumulator r: column (r & 3) + 8 (r >> 2) + 4 lh, row lr
+        *(sum4*)(mine + lr * PITCH + (i * 32 + 8 * q + 4 * lh) * 4) =
+            sum4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    if (lh == 0) *(float*)(mine + lr * PITCH + NI * 128) = sxr[j];
+  };
+#pragma unroll 1
+  for (int j = 0; j < MJ; ++j) {
+    if (j == 0) stage_out(std::integral_constant<int, 0>{});
+    if constexpr (MJ > 1)
+      if (j == 1) stage_out(std::integral_constant<int, 1>{});
+    if constexpr (MJ > 2)
+      if (j == 2) stage_out(std::integral_constant<int, 2>{});
+    if constexpr (MJ > 3)
+      if (j == 3) stage_out(std::integral_constant<int, 3>{});
+    asm volatile("" ::: "memory");
+    const int mj = m0 + (wm * MJ + j) * 32 + cr;
+#pragma unroll 1
+    for (int t = 0; t < 32; t += RPI * U) {
+      v4f v[U], r[U];
+      float sx[U];
+      if (a.vec && a.res) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int m = mj + t + u * RPI;
+          r[u] = v4f{0.f, 0.f, 0.f, 0.f};
+          if (m < m1 && in) r[u] = residual4(a, m, cn);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int8_t* p = mine + (t + u * RPI + cr) * PITCH;
+        const sum4 c = *(const sum4*)(p + 16 * (lane % LPR));
+        v[u] = v4f{(float)c[0], (float)c[1], (float)c[2], (float)c[3]};
+        sx[u] = *(const float*)(p + NI * 128);
+      }
+      with_act(a.act, [&](auto act) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = scaled4<decltype(act)::value>(v[u], sx[u], ws, bias);
+      });
+      if (a.vec) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int m = mj + t + u * RPI;
+          if (m < m1 && in) put4(a, m, cn, a.res ? v[u] + r[u] : v[u]);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int m = mj + t + u * RPI;
+          if (m < m1 && in) put4_any(a, m, cn, v[u]);
+        }
+      }
+    }
+    asm volatile("" ::: "memory");
+  }
+}
+
+// row tiles of BM that the rows can need; grouped: each expert adds at most
+// one part-filled tile, and no tile is empty
+long row_tiles(const LinearArgs& a, int BM) {
+  if (!a.E) return (a.M + BM - 1) / BM;
+  const long t = a.M / BM + a.E;
+  return t < a.M ? t : a.M;
+}
+
+template <bool F8, int WN, int WM, int NI, int MJ, int KB, int SLOTS, int WPE>
+hipError_t launch_tile(const LinearArgs& a, hipStream_t s) {
+  constexpr int TN = 32 * WN * NI, TM = 32 * WM * MJ;
+  const long nbn = (a.N + TN - 1) / TN, nbm = row_tiles(a, TM);
+  if (!grid_fits(nbm * nbn, WN * WM * 64)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((linear_tile_kernel<F8, WN, WM, NI, MJ, KB, SLOTS, WPE>), dim3((unsigned)(nbm * nbn)),
+                     dim3(WN * WM * 64), 0, s, a, (int)nbm, (int)nbn);
+  return hipGetLastError();
+}
+
+template <bool F8, int MI, int NJ, int WK, int U>
 hipError_t launch_direct(const LinearArgs& a, hipStream_t s) {
   constexpr int BM = 16 * MI, BN = 16 * NJ;
   const long nbn = (a.N + BN - 1) / BN;
-  // grouped: each expert adds at most one part-filled tile, and no tile is empty
-  long mt = (a.M + BM - 1) / BM;
-  if (a.E) {
-    mt = a.M / BM + a.E;
-    if (mt > a.M) mt = a.M;
-  }
+  const long mt = row_tiles(a, BM);
   if (!grid_fits(mt * nbn, WK * 64)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((linear_direct_kernel<F8, MI, NJ, WK>), dim3((unsigned)(mt * nbn)), dim3(WK * 64), 0, s, a);
+  hipLaunchKernelGGL((linear_direct_kernel<F8, MI, NJ, WK, U>), dim3((unsigned)(mt * nbn)), dim3(WK * 64), 0, s, a,
+                     (int)mt);
   return hipGetLastError();
+}
+
+int num_cus() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0)
+      v = 256;
+    return v;
+  }();
+  return n;
+}
+
+// Which kernel.  Measured on one box (us, weights from memory, s8 / e4m3):
+//   M x N x K           direct 16 / 32 / 64   64 x 64   128 x 128   256 x 256
+//   1 x 4096 x 4096      5.8 / 8.9 / 15          13        32
+//   16 x 4096 x 4096     6.8 / 10 / 16           13        32          62
+//   64 x 4096 x 4096      17 / 11 / 21           14        34
+//   256 x 4096 x 4096     59 / 32 / 21        14.8 / 13.6  34          67
+//   512 x 4096 x 4096    115 / 61 / 34        21.4 / 20.7  34          66
+//   1003 x 5000 x 2736   137 / 80 / 50          47 / 44    37        62 / 58
+//   2048 x 4096 x 4096                          70 / 65   45 / 43    67 / 60
+//   4096 x 4096 x 4096                         129 / 118  84 / 81    74 / 68
+//   8192 x 8192 x 8192                         910 / 810 566 / 493  497 / 430
+// A tile's stage costs what its DMA and its chain of steps take, nearly the
+// same whatever else runs: so the tiles are compared by rounds of workgroups
+// times a round's cost per K (per 1024 of K, first with one workgroup per CU,
+// then with two).
+struct TileCost {
+  int tn, tm, per_cu;
+  float one, two, fixed;
+};
+constexpr TileCost kTiles[3] = {{64, 64, 2, 2.9f, 4.4f, 3.f}, {128, 128, 2, 6.5f, 10.f, 4.f}, {256, 256, 1, 16.f, 16.f, 7.f}};
+
+// rows' tiles of height tm; grouped: as if each expert's last one were half full
+float tiles_of_rows(const LinearArgs& a, int tm) {
+  if (!a.E) return (float)((a.M + tm - 1) / tm);
+  const float t = (float)a.M / tm + 0.5f * a.E;
+  return t < a.M ? t : (float)a.M;
+}
+
+int best_tile(const LinearArgs& a) {
+  int best = 0;
+  float least = 0.f;
+  const float cus = (float)num_cus();
+  for (int i = 0; i < 3; ++i) {
+    const TileCost& t = kTiles[i];
+    const float wgs = tiles_of_rows(a, t.tm) * (float)((a.N + t.tn - 1) / t.tn), round = cus * t.per_cu;
+    const float rounds = __builtin_floorf(wgs / round), rest = wgs - rounds * round;
+    const float k = a.K / 1024.f;
+    const float c = rounds * (t.two * k + t.fixed) + (rest <= 0.f ? 0.f : (rest <= cus ? t.one : t.two) * k + t.fixed);
+    if (i == 0 || c < least) {
+      least = c;
+      best = i;
+    }
+  }
+  return best;
+}
+
+template <bool F8>
+hipError_t launch_linear_any(const LinearArgs& a, bool dma, hipStream_t s) {
+  const float rows = a.E ? (float)a.M / a.E : (float)a.M;  // rows that share weights
+  const float wgs = tiles_of_rows(a, 64) * (float)((a.N + 63) / 64);
+  if (rows <= 16.f)
+    return a.K < 8192 ? launch_direct<F8, 1, 1, 4, 4>(a, s) : launch_direct<F8, 1, 1, 8, 4>(a, s);
+  // half the chip's CUs are not enough to pull the weights by 64 x 64 tiles
+  if (dma && (!F8 || a.bf16) && wgs >= 0.5f * num_cus()) switch (best_tile(a)) {
+      case 0: return launch_tile<F8, 2, 2, 1, 1, 128, 5, 2>(a, s);
+      case 1: return launch_tile<F8, 2, 2, 2, 2, 128, 2, 2>(a, s);
+      default: return launch_tile<F8, 2, 2, 4, 4, 128, 2, 1>(a, s);
+    }
+  if (wgs < (float)num_cus()) return launch_direct<F8, 2, 2, 4, 4>(a, s);
+  return launch_direct<F8, 4, 4, 4, 2>(a, s);
 }
 
 template <bool F8>
 int linear_any(const char* who, const dlq_linear_desc* d, int E, const int32_t* off, const void* x, const float* xs,
                const void* w, const float* ws, const float* bias, const void* res, void* y, void* stream) {
-  const std::string p = std::string(who) + ": ";
-  if (!d || d->M < 0 || d->N < 0 || d->K < 0) return fail(DLQ_ERR_ARG, p + "bad shape");
-  if (d->K > 131071) return fail(DLQ_ERR_ARG, p + "K above 131071");
-  if (d->act < DLQ_ACT_NONE || d->act > DLQ_ACT_SILU) return fail(DLQ_ERR_ARG, p + "bad act");
-  if (d->out_type != DLQ_T_F32 && d->out_type != DLQ_T_BF16) return fail(DLQ_ERR_ARG, p + "bad out_type");
-  if (d->ldx < d->K || d->ldw < d->K) return fail(DLQ_ERR_ARG, p + "row stride below K");
-  if (d->ldy < d->N || (res && d->ldr < d->N)) return fail(DLQ_ERR_ARG, p + "row stride below N");
-  if (E < 0 || E > 65535) return fail(DLQ_ERR_ARG, p + "experts outside 0..65535");
+  const auto bad = [&](const char* what) { return fail(DLQ_ERR_ARG, std::string(who) + ": " + what); };
+  if (!d || d->M < 0 || d->N < 0 || d->K < 0) return bad("bad shape");
+  if (d->K > 131071) return bad("K above 131071");
+  if (d->act < DLQ_ACT_NONE || d->act > DLQ_ACT_SILU) return bad("bad act");
+  if (d->out_type != DLQ_T_F32 && d->out_type != DLQ_T_BF16) return bad("bad out_type");
+  if (d->ldx < d->K || d->ldw < d->K) return bad("row stride below K");
+  if (d->ldy < d->N || (res && d->ldr < d->N)) return bad("row stride below N");
+  if (E < 0 || E > 65535) return bad("experts outside 0..65535");
   if (d->M == 0 || d->N == 0 || (off && E == 0)) return DLQ_OK;
-  if (!ws || !y || (d->K && (!x || !w))) return fail(DLQ_ERR_ARG, p + "null pointer");
+  if (!ws || !y || (d->K && (!x || !w))) return bad("null pointer");
   const uintptr_t es = d->out_type == DLQ_T_BF16 ? 2 : 4;
   if (((uintptr_t)xs | (uintptr_t)ws | (uintptr_t)bias | (uintptr_t)off) % 4 || ((uintptr_t)y | (uintptr_t)res) % es)
-    return fail(DLQ_ERR_ARG, p + "pointer not aligned to its element type");
-  if (res == y && res && d->ldr != d->ldy) return fail(DLQ_ERR_ARG, p + "residual is y with another row stride");
+    return bad("pointer not aligned to its element type");
+  if (res == y && res && d->ldr != d->ldy) return bad("residual is y with another row stride");
   LinearArgs a;
   a.x = (const int8_t*)x;
   a.w = (const int8_t*)w;
@@ -282,11 +753,13 @@ int linear_any(const char* who, const dlq_linear_desc* d, int E, const int32_t* 
   a.act = d->act;
   a.bf16 = d->out_type == DLQ_T_BF16;
   a.vec = ((uintptr_t)ws | (uintptr_t)bias) % 16 == 0 && ((uintptr_t)y | (uintptr_t)res) % (4 * es) == 0 &&
-          d->ldy % 4 == 0 && (!res || d->ldr % 4 == 0) && (E <= 1 || d->N % 4 == 0);
+          d->N % 4 == 0 && d->ldy % 4 == 0 && (!res || d->ldr % 4 == 0);
   a.E = E;
   a.off = off;
-  const hipError_t e = launch_direct<F8, 1, 1, 4>(a, (hipStream_t)stream);
-  return e == hipSuccess ? DLQ_OK : fail(DLQ_ERR_LAUNCH, p + "launch: " + hipGetErrorString(e));
+  const bool dma = ((uintptr_t)x | (uintptr_t)w) % 16 == 0 && d->K % 16 == 0 && d->ldx % 16 == 0 && d->ldw % 16 == 0 &&
+                   d->ldx <= (1 << 22) && d->ldw <= (1 << 22);  // a tile's offsets fit 32 bits
+  const hipError_t e = launch_linear_any<F8>(a, dma, (hipStream_t)stream);
+  return e == hipSuccess ? DLQ_OK : fail(DLQ_ERR_LAUNCH, std::string(who) + " launch: " + hipGetErrorString(e));
 }
 
 }  // namespace

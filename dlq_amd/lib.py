@@ -188,6 +188,17 @@ def ptr(t) -> int | None:
     return t.ctypes.data  # numpy
 
 
+# handle of device `index`'s current stream: the interpreter's own accessor, a
+# Stream object costs 2.6 us per call (a launch 3.4)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(index: int) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
 def stream_handle(stream=None) -> int | None:
     if stream is None:
         stream = torch.cuda.current_stream()

@@ -19,7 +19,7 @@ import numpy as np
 import torch
 
 from .lib import (DLQ_ACT, DLQ_OUT_F32, DLQ_OUT_S8, DLQ_OUT_S32, DLQ_T_BF16, DLQ_T_F32, ConvDesc, LinearDesc,
-                  check, lib, ptr, stream_handle)
+                  check, lib, ptr, raw_stream, stream_handle)
 
 
 def out_dim(n, k, s, p):
@@ -454,18 +454,21 @@ def block_l1_f8(x: torch.Tensor, w1: torch.Tensor, alpha1: torch.Tensor, beta1: 
 _TYPES = {torch.float32: DLQ_T_F32, torch.bfloat16: DLQ_T_BF16}
 
 
-def _rows(t: torch.Tensor, name: str, dtypes, rows=None, cols=None) -> int:
-    """Checks a row-strided CUDA matrix; its row stride in elements."""
+def _rows(t: torch.Tensor, name: str, dtypes, rows=None, cols=None):
+    """Checks a row-strided CUDA matrix: its rows, columns and row stride in elements."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
         raise TypeError(f"{name}: expected a CUDA tensor of {' or '.join(map(str, dtypes))}")
-    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [{'rows' if rows is None else rows}, "
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (cols is not None and shape[1] != cols):
+        raise ValueError(f"{name}: shape {tuple(shape)}, expected [{'rows' if rows is None else rows}, "
                          f"{'cols' if cols is None else cols}]")
-    r, c = t.shape
-    ld = t.stride(0) if r > 1 else c
-    if (c > 1 and t.stride(1) != 1) or ld < c:
+    r, c = shape
+    ld, unit = t.stride()
+    if r <= 1:
+        ld = c
+    if (c > 1 and unit != 1) or ld < c:
         raise ValueError(f"{name}: rows must have unit stride and not overlap, strides {t.stride()}")
-    return ld
+    return r, c, ld
 
 
 def _vector(t, name: str, dtype, shape):
@@ -481,23 +484,23 @@ def _vector(t, name: str, dtype, shape):
 
 def _launch(what: str, fn, tensors, *args) -> None:
     """fn(*args, stream) on the tensors' one device and its current stream."""
-    dev = tensors[0].device
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, stream_handle()), what)
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, stream_handle()), what)
+            rc = fn(*args, raw_stream(dev))
+    check(rc, what)
 
 
 def _quantize_rows_dyn(what, fn, dtype, x, ld):
-    ldx = _rows(x, "x", _TYPES)
-    rows, cols = x.shape
-    q = torch.empty((rows, cols if ld is None else ld), dtype=dtype, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    _launch(what, fn, (x,), x.data_ptr(), _TYPES[x.dtype], rows, cols, ldx, q.data_ptr(), q.shape[1],
+    rows, cols, ldx = _rows(x, "x", _TYPES)
+    q = x.new_empty((rows, cols if ld is None else ld), dtype=dtype)
+    scale = x.new_empty(rows, dtype=torch.float32)
+    _launch(what, fn, (x,), x.data_ptr(), _TYPES[x.dtype], rows, cols, ldx, q.data_ptr(), cols if ld is None else ld,
             scale.data_ptr())
     return q, scale
 
@@ -521,31 +524,38 @@ def _linear(what, fn, code, x, w, x_scale, w_scale, bias, act, residual, out_dty
         out_dtype = out.dtype
     if out_dtype not in _TYPES:
         raise TypeError("output must be torch.float32 or torch.bfloat16")
-    ldx = _rows(x, "x", (code,))
-    M, K = x.shape
+    M, K, ldx = _rows(x, "x", (code,))
     if offsets is None:
-        ldw = _rows(w, "w", (code,), cols=K)
-        N, lead = w.shape[0], ()
+        N, _, ldw = _rows(w, "w", (code,), cols=K)
+        per_column = (N,)
     else:
         if not (isinstance(w, torch.Tensor) and w.is_cuda and w.dtype == code and w.dim() == 3 and w.is_contiguous()):
             raise TypeError(f"w: expected a contiguous CUDA tensor [E, N, K] of {code}")
         E, N, ldw = w.shape
-        lead = (E,)
+        per_column = (E, N)
         if ldw != K:
             raise ValueError(f"w: shape {tuple(w.shape)}, expected [E, N, {K}]")
     if w_scale is None:
         raise TypeError("w_scale is required")
     sx = _vector(x_scale, "x_scale", torch.float32, (M,))
-    sw = _vector(w_scale, "w_scale", torch.float32, lead + (N,))
-    sb = _vector(bias, "bias", torch.float32, lead + (N,))
-    ldr = 0 if residual is None else _rows(residual, "residual", (out_dtype,), M, N)
+    sw = _vector(w_scale, "w_scale", torch.float32, per_column)
+    sb = _vector(bias, "bias", torch.float32, per_column)
+    res, ldr = None, 0
+    if residual is not None:
+        ldr = _rows(residual, "residual", (out_dtype,), M, N)[2]
+        res = residual.data_ptr()
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
-    d = LinearDesc(M, N, K, ldx, ldw, _rows(out, "out", (out_dtype,), M, N), ldr, DLQ_ACT[act], _TYPES[out_dtype])
-    args = (x.data_ptr(), sx, w.data_ptr(), sw, sb, None if residual is None else residual.data_ptr(), out.data_ptr())
-    if offsets is not None:
-        args = (E, _vector(offsets, "offsets", torch.int32, (E + 1,))) + args
-    _launch(what, fn, (x, w, x_scale, w_scale, bias, residual, out, offsets), C.byref(d), *args)
+        out, ldy = x.new_empty((M, N), dtype=out_dtype), N
+    else:
+        ldy = _rows(out, "out", (out_dtype,), M, N)[2]
+    d = C.byref(LinearDesc(M, N, K, ldx, ldw, ldy, ldr, DLQ_ACT[act], _TYPES[out_dtype]))
+    if offsets is None:
+        _launch(what, fn, (x, w, x_scale, w_scale, bias, residual, out), d, x.data_ptr(), sx, w.data_ptr(), sw, sb, res,
+                out.data_ptr())
+    else:
+        at = _vector(offsets, "offsets", torch.int32, (E + 1,))
+        _launch(what, fn, (x, w, x_scale, w_scale, bias, residual, out, offsets), d, E, at, x.data_ptr(), sx,
+                w.data_ptr(), sw, sb, res, out.data_ptr())
     return out
 
 
@@ -605,15 +615,14 @@ def logprobs(x: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0) 
     """Log probabilities of fp32 / bf16 logits [rows, K] (dlq_logprobs): of
     tokens int32 [rows] (0 where negative), the rows' entropy, and the `top`
     (<= 64) largest with their indices, equal ones by ascending index."""
-    ldx = _rows(x, "x", _TYPES)
-    rows, K = x.shape
+    rows, K, ldx = _rows(x, "x", _TYPES)
     t = _vector(tokens, "tokens", torch.int32, (rows,))
-    lp = None if tokens is None else torch.empty(rows, dtype=torch.float32, device=x.device)
-    ent = torch.empty(rows, dtype=torch.float32, device=x.device)
-    ti = torch.empty((rows, top), dtype=torch.int32, device=x.device) if top > 0 else None
-    tl = torch.empty((rows, top), dtype=torch.float32, device=x.device) if top > 0 else None
+    lp = None if tokens is None else x.new_empty(rows, dtype=torch.float32)
+    ent = x.new_empty(rows, dtype=torch.float32)
+    ti = x.new_empty((rows, top), dtype=torch.int32) if top > 0 else None
+    tl = x.new_empty((rows, top), dtype=torch.float32) if top > 0 else None
     nb = lib.dlq_logprobs_workspace_bytes(rows, K, top)
-    ws = torch.empty(nb, dtype=torch.uint8, device=x.device) if nb else None
+    ws = x.new_empty(nb, dtype=torch.uint8) if nb else None
     _launch("logprobs", lib.dlq_logprobs, (x, tokens), x.data_ptr(), _TYPES[x.dtype], rows, K, ldx, t, top, ptr(lp),
             ent.data_ptr(), ptr(ti), ptr(tl), ptr(ws), nb)
     return LogProbs(lp, ent, ti, tl)

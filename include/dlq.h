@@ -549,7 +549,10 @@ typedef struct dlq_linear_desc {
  *   v = fma(float(acc), x_scale[m] * w_scale[n], bias[n]),
  *   acc = sum_k x[m][k] * w[n][k]
  * (s8: the exact int32 sum; e4m3: exact products summed in fp32, in a fixed
- * order).  x_scale, bias and residual may be NULL (1, 0, none); w_scale not.
+ * order; with bf16 output larger products take the fp8 matrix instructions,
+ * which cut the products of 8 consecutive k 13 bits below the largest of them:
+ * acc is then off by up to 7 * 2^-13 sum over those 8s of max |x w|, on normal
+ * data 1.4e-5 of the result).  x_scale, bias and residual may be NULL (1, 0, none); w_scale not.
  * w is used as stored: no packing.  residual may be y itself (same ld); any
  * other overlap of y with an input is not allowed.  K <= 131071 (an int32 sum
  * of 2^14-sized products); K = 0 gives acc = 0. */

@@ -7,7 +7,11 @@ Tolerances (u = 2^-24, the half step of fp32; bf16's is 2^-8):
    products) is off by at most 8 u |v|; the residual's add and the output's
    rounding are half a step each.  e4m3: products are exact and fp32 sums of K
    of them take K/32 matrix steps of up to 32 additions' depth and the join of
-   at most 16 slices, so (K/32 + 48) u sum |x w| more.
+   at most 16 slices, so (K/32 + 48) u sum |x w| more.  With bf16 output the
+   fp8 matrix instructions may be taken: the products of 8 consecutive k lose
+   what lies 13 bits below the largest one's exponent, so each of the 7 others
+   is off by at most 2^-13 of it: 7 * 2^-13 sum over the 8s of max |x w| more
+   (bounded here by max |x| max |w|).
  * codes and scales are compared exactly: every step is one IEEE operation.
  * log probabilities: see lp_bounds.
 """
@@ -57,6 +61,9 @@ def product64(x, w, xs, ws, bias, act, res, out_dtype):
     tol = 1.13 * U * (2 * acc.abs() + v.abs()) + 8 * U * v.abs() + U * y.abs() + 1e-30
     if x.dtype == torch.uint8:
         tol = tol + 1.13 * U * (x.shape[1] / 32 + 48) * (vx.abs() @ vw.abs().T) * s
+        if out_dtype == torch.bfloat16:
+            g = [torch.nn.functional.pad(v.abs(), (0, -v.shape[1] % 8)).view(len(v), -1, 8).amax(2) for v in (vx, vw)]
+            tol = tol + 1.13 * 7 * 2.0 ** -13 * (g[0] @ g[1].T) * s
     return y, tol + HALF[out_dtype] * (y.abs() + tol)
 
 
@@ -93,7 +100,8 @@ def dev(t):
 
 SHAPES = [(1, 1, 1), (1, 16, 64), (1, 4096, 512), (3, 17, 31), (2, 129, 1000), (16, 48, 128), (17, 64, 129),
           (33, 100, 255), (64, 128, 1024), (65, 257, 300), (128, 128, 256), (100, 1000, 512), (130, 384, 640),
-          (257, 260, 1040), (300, 513, 144), (512, 512, 2048)]
+          (257, 260, 1040), (300, 513, 144), (512, 512, 2048), (700, 1500, 272), (130, 8200, 144), (1100, 2050, 128),
+          (2500, 4000, 48), (2500, 4001, 400), (1500, 3000, 656), (2500, 4000, 1104)]
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
