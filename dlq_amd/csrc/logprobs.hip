@@ -77,23 +77,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// A wave's 64 values joined by f, the same in every lane: within rows of 16,
-// then across them, by data-parallel primitives (no LDS round trips).  none:
-// f(none, v) = v.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_move(int v, int none) {
-  return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false);
-}
-template <typename F>
-__device__ __forceinline__ int wave_join(int v, int none, F f) {
-  v = f(v, dpp_move<0x111, 0xf>(v, none));  // row_shr 1, 2, 4, 8
-  v = f(v, dpp_move<0x112, 0xf>(v, none));
-  v = f(v, dpp_move<0x114, 0xf>(v, none));
-  v = f(v, dpp_move<0x118, 0xf>(v, none));
-  v = f(v, dpp_move<0x142, 0xa>(v, none));  // row_bcast 15, 31
-  v = f(v, dpp_move<0x143, 0xc>(v, none));
-  return __builtin_amdgcn_readlane(v, 63);
-}
 __device__ __forceinline__ float wave_max(float v) {
   return __int_as_float(wave_join(__float_as_int(v), __float_as_int(-INFINITY), [](int p, int q) {
     return __float_as_int(fmaxf(__int_as_float(p), __int_as_float(q)));

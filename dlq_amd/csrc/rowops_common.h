@@ -35,6 +35,24 @@ __device__ __forceinline__ unsigned bf_pack(float a, float b) {
   return __builtin_bit_cast(unsigned, r);
 }
 
+// A wave's 64 values joined by f, the same in every lane: within rows of 16,
+// then across them, by data-parallel primitives (no LDS round trips).  none:
+// f(none, v) = v.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_move(int v, int none) {
+  return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false);
+}
+template <typename F>
+__device__ __forceinline__ int wave_join(int v, int none, F f) {
+  v = f(v, dpp_move<0x111, 0xf>(v, none));  // row_shr 1, 2, 4, 8
+  v = f(v, dpp_move<0x112, 0xf>(v, none));
+  v = f(v, dpp_move<0x114, 0xf>(v, none));
+  v = f(v, dpp_move<0x118, 0xf>(v, none));
+  v = f(v, dpp_move<0x142, 0xa>(v, none));  // row_bcast 15, 31
+  v = f(v, dpp_move<0x143, 0xc>(v, none));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 // A launch's blocks * threads must stay below 2^32 (the dispatch packet's grid
 // size is 32 bits of work-items).
 inline bool grid_fits(long long blocks, int threads) { return blocks * threads < (1LL << 32); }

@@ -305,7 +305,8 @@ def quant_reference(x, t, ld):
 @pytest.mark.parametrize("rows,cols,ld,pad", [(1, 1, 1, 0), (1, 1, 16, 3), (3, 7, 7, 0), (5, 64, 64, 0), (2, 513, 520, 1),
                                               (9, 1000, 1008, 0), (4, 2048, 2048, 8), (3, 4097, 4112, 0),
                                               (2, 8192, 8192, 0), (3, 16384, 16384, 0), (2, 16391, 16400, 5),
-                                              (2, 40000, 40001, 0), (70, 300, 300, 4)])
+                                              (2, 40000, 40001, 0), (70, 300, 300, 4),
+                                              (2, 65536, 65536, 0), (2, 70001, 70010, 3)])
 def test_quantize_rows_dyn(gpu, t, xt, rows, cols, ld, pad):
     from dlq_amd import ops
     rng = np.random.default_rng([rows, cols])
