@@ -23,6 +23,7 @@ struct LinearArgs {
   void* y;
   int M, N, K;
   size_t ldx, ldw, ldy, ldr;
+  int odd;             // some row of x or w does not start on a dword
   int act, bf16, vec;  // vec: y, res, ws and bias take aligned 4-element accesses
   int E;               // 0: one product over all rows
   const int* off;      // [E + 1], E > 0
@@ -203,7 +204,7 @@ struct Mma<true> {
 // workgroup, its WK waves each take a slice of K and join their sums in LDS
 // (in wave order).  Lane l holds row l & 15, 16 bytes at 16 (l >> 4) of every
 // 64: the order of K within a step is free as long as both operands agree.
-template <bool F8, int MI, int NJ, int WK, int U>
+template <bool F8, bool ODD, int MI, int NJ, int WK, int U>
 __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs a, int nbm) {
   typedef Mma<F8> MM;
   typedef typename MM::acc_t acc_t;
@@ -237,28 +238,36 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
   const int steps = (a.K + KB - 1) / KB, full = a.K / KB;
   const int s0 = (int)((long)steps * wave / WK), s1 = (int)((long)steps * (wave + 1) / WK);
   // U steps' loads are on their way while U others are multiplied
-  v4i rx[2][U][MI], rw[2][U][NJ];
+  Raw16<ODD> rx[2][U][MI], rw[2][U][NJ];
   auto load = [&](int b, int s) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) rw[b][u][j] = *(const v4i_any*)(wp[j] + (size_t)(s + u) * KB);
+      for (int j = 0; j < NJ; ++j) rw[b][u][j].load(wp[j] + (size_t)(s + u) * KB);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) rx[b][u][i] = *(const v4i_any*)(xp[i] + (size_t)(s + u) * KB);
+      for (int i = 0; i < MI; ++i) rx[b][u][i].load(xp[i] + (size_t)(s + u) * KB);
     }
   };
-  auto multiply = [&](int b, int n) __attribute__((always_inline)) {
+  auto product = [&](const v4i* vx, const v4i* vw) __attribute__((always_inline)) {
+    typename MM::frag fx[MI], fw[NJ];
 #pragma unroll
-    for (int u = 0; u < n; ++u) {
-      typename MM::frag fx[MI], fw[NJ];
+    for (int i = 0; i < MI; ++i) fx[i] = MM::prep(vx[i]);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fx[i] = MM::prep(rx[b][u][i]);
+    for (int j = 0; j < NJ; ++j) fw[j] = MM::prep(vw[j]);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) fw[j] = MM::prep(rw[b][u][j]);
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+      for (int j = 0; j < NJ; ++j) acc[i][j] = MM::go(fw[j], fx[i], acc[i][j]);
+  };
+  auto multiply = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = MM::go(fw[j], fx[i], acc[i][j]);
+    for (int u = 0; u < U; ++u) {
+      v4i vx[MI], vw[NJ];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) vx[i] = rx[b][u][i].get(xp[i]);  // a step is a multiple of a dword
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) vw[j] = rw[b][u][j].get(wp[j]);
+      product(vx, vw);
     }
   };
   const int sf = s1 < full ? s1 : full;
@@ -266,26 +275,27 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
   if (s + U <= sf) load(0, s);
   for (; s + 3 * U <= sf; s += 2 * U) {
     load(1, s + U);
-    multiply(0, U);
+    multiply(0);
     load(0, s + 2 * U);
-    multiply(1, U);
+    multiply(1);
   }
   if (s + 2 * U <= sf) {
     load(1, s + U);
-    multiply(0, U);
-    multiply(1, U);
+    multiply(0);
+    multiply(1);
     s += 2 * U;
   } else if (s + U <= sf) {
-    multiply(0, U);
+    multiply(0);
     s += U;
   }
   for (; s < s1; ++s) {
-    const int k = s * KB, avail = s < full ? 16 : a.K - k - 16 * lg;  // the end of K: zeros past it
+    const int k = s * KB, avail = a.K - k - 16 * lg;  // the end of K: zeros past it
+    v4i vx[MI], vw[NJ];
 #pragma unroll
-    for (int i = 0; i < MI; ++i) rx[0][0][i] = load_codes16(xp[i] + k, avail);
+    for (int i = 0; i < MI; ++i) vx[i] = load_tail16<ODD>(xp[i] + k, avail, k + 16 * lg);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) rw[0][0][j] = load_codes16(wp[j] + k, avail);
-    multiply(0, 1);
+    for (int j = 0; j < NJ; ++j) vw[j] = load_tail16<ODD>(wp[j] + k, avail, k + 16 * lg);
+    product(vx, vw);
   }
 #pragma unroll
   for (int i = 0; i < MI; ++i)
@@ -338,22 +348,27 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
 // e4m3 here uses the fp8 matrix instructions, whose cut products (see Mma) are
 // off by up to 7 * 2^-13 of the largest of each 8: 1.4e-5 of the result on
 // normal data, which bf16's rounding (2^-9) hides; only bf16 outputs come here.
-template <bool F8>
-struct TileMma {
+template <bool F8, int NV>
+struct TileMma {  // a fragment: NV 16-byte reads, 32 K bytes of a row each
   typedef v16i acc_t;
   typedef v4i sum4;
-  static constexpr int NV = 1;  // 16-byte reads per fragment
   static __device__ __forceinline__ v16i go(const v4i* a, const v4i* b, v16i c) {
-    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a[0], b[0], c, 0, 0, 0);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) c = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[v], b[v], c, 0, 0, 0);
+    return c;
   }
 };
-template <>
-struct TileMma<true> {
+template <int NV>
+struct TileMma<true, NV> {
+  static_assert(NV % 2 == 0, "64 K bytes per instruction");
   typedef v16f acc_t;
   typedef v4f sum4;
-  static constexpr int NV = 2;
   static __device__ __forceinline__ v16f go(const v4i* a, const v4i* b, v16f c) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat8(a[0], a[1]), cat8(b[0], b[1]), c, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+    for (int v = 0; v < NV; v += 2)
+      c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat8(a[v], a[v + 1]), cat8(b[v], b[v + 1]), c, 0, 0, 0, 0, 0,
+                                                          0);
+    return c;
   }
 };
 
@@ -366,12 +381,12 @@ __device__ __forceinline__ const int8_t* uniform(const int8_t* p) {
   return (const int8_t*)((unsigned long long)hi << 32 | lo);
 }
 
-template <bool F8, int WN, int WM, int NI, int MJ, int KB, int SLOTS, int WPE>
+template <bool F8, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE>
 __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const LinearArgs a, int nbm, int nbn) {
-  typedef TileMma<F8> MM;
+  typedef TileMma<F8, NV> MM;
   typedef typename MM::acc_t acc_t;
   typedef typename MM::sum4 sum4;
-  constexpr int NW = WN * WM, TN = 32 * WN * NI, TM = 32 * WM * MJ, NV = MM::NV;
+  constexpr int NW = WN * WM, TN = 32 * WN * NI, TM = 32 * WM * MJ;
   constexpr int SPS = KB / 32 / NV;                        // K steps of a stage
   constexpr int CPR = KB / 16, RPP = 64 / CPR;             // chunks of a row, rows of a 1 KiB piece
   constexpr int SLOT = (TN + TM) * KB;
@@ -421,9 +436,34 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
   const int nst = (a.K + KB - 1) / KB, full = a.K / KB;
   const int8_t* zsrc = g_zero_linear;
   asm volatile("" : "+s"(zsrc));
-  // piece r of stage st into a slot; whole: all of the stage lies within K
+  const auto slot_at = [&](int slot, int r) __attribute__((always_inline)) {
+    return slot * SLOT + (r < PW ? 0 : TN * KB) + (wave + NW * (r < PW ? r : r - PW)) * 1024;
+  };
+  // piece r of stage st into a slot; whole: all of the stage lies within K.
+  // REG (rows that are not 16-byte aligned, which the DMA cannot take): the
+  // piece of the stage before goes from registers into the slot, and the
+  // stage's own is loaded into them.
+  Raw16<true> held[REG ? PP : 1];  // pieces at the end of K: in place already
+  auto fetch = [&](int st, int r, bool whole) __attribute__((always_inline)) {
+    const int8_t* base = (r < PW ? wbase : xbase) + (size_t)st * KB;
+    const unsigned v = r < PW ? vw[r < PW ? r : 0] : vx[r < PW ? 0 : r - PW];
+    if (whole || st < full) {
+      held[r].load(base + v);
+    } else {
+      held[r].d = load_tail16<true>(base + v, a.K - st * KB - 16 * chunk, st * KB + 16 * chunk);  // zeros past K
+    }
+  };
+  auto stash = [&](int st, int slot, int r, bool whole) __attribute__((always_inline)) {
+    const int8_t* p = (r < PW ? wbase : xbase) + (r < PW ? vw[r < PW ? r : 0] : vx[r < PW ? 0 : r - PW]);
+    *(v4i*)(lds + slot_at(slot, r) + lane * 16) = whole || st < full ? held[r].get(p) : held[r].d;
+  };
   auto issue = [&](int st, int slot, int r, bool whole) __attribute__((always_inline)) {
-    const unsigned to = lds32 + slot * SLOT + (r < PW ? 0 : TN * KB) + (wave + NW * (r < PW ? r : r - PW)) * 1024;
+    if constexpr (REG) {
+      stash(st, slot, r, whole);
+      fetch(st + 1, r, whole);
+      return;
+    }
+    const unsigned to = lds32 + slot_at(slot, r);
     const int8_t* base = (r < PW ? wbase : xbase) + (size_t)st * KB;
     const unsigned v = r < PW ? vw[r < PW ? r : 0] : vx[r < PW ? 0 : r - PW];
     if (whole || st < full)
@@ -450,19 +490,21 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
     else
       fw[b][f - MJ][v] = *(const v4i*)(p + ((wn * NI + f - MJ) * 32 + lr) * KB);
   };
-  // one step's matrix instructions on buffer b; behind instruction t come reads
-  // of the next step (rslot >= 0) and DMA pieces of stage dst (dst >= 0)
+  // one step's matrix instructions on buffer b; between them, in its first
+  // half, the reads of the next step (rslot >= 0), and DMA pieces of stage dst
+  // (dst >= 0)
   auto step = [&](int b, int rslot, int rstep, int dst, int dslot, bool whole) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < NM; ++t) {
       const int i = t / MJ, j = t % MJ;
-      acc[i][j] = MM::go(fw[b][i], fx[b][j], acc[i][j]);
-      __builtin_amdgcn_sched_barrier(0);
       if (rslot >= 0) {
 #pragma unroll
         for (int q = 0; q < NR; ++q)
-          if (q * NM / NR == t) read(rslot, rstep, b ^ 1, q);
+          if (q * NM / (2 * NR) == t) read(rslot, rstep, b ^ 1, q);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      acc[i][j] = MM::go(fw[b][i], fx[b][j], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
       if (dst >= 0) {
 #pragma unroll
         for (int r = 0; r < PP; ++r)
@@ -477,7 +519,9 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
   auto stage = [&](int s, int slot, int next, int b0, bool whole) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k + 1 < SPS; ++k) step((b0 + k) & 1, slot, k + 1, -1, 0, false);
-    if (whole) {
+    if (REG) {  // this wave's writes of stage s + 1 are done; its loads go on
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    } else if (whole) {
       wait_vm_const<PP*(SLOTS - 2)>();  // and lgkmcnt(0)
     } else {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -487,6 +531,10 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
     step((b0 + SPS - 1) & 1, next, 0, s + SLOTS, slot, whole);
   };
 
+  if constexpr (REG) {
+#pragma unroll
+    for (int r = 0; r < PP; ++r) fetch(0, r, false);
+  }
 #pragma unroll
   for (int st = 0; st < SLOTS; ++st)
 #pragma unroll
@@ -507,7 +555,9 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
     const int m = m0 + (wm * MJ + j) * 32 + lr;
     sxr[j] = a.xs && m < m1 ? a.xs[m] : 1.f;
   }
-  if (nst >= SLOTS)
+  if (REG)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  else if (nst >= SLOTS)
     wait_vm_const<PP*(SLOTS - 1)>();  // stage 0 has landed, the others may be under way
   else
     wait_vm0();
@@ -521,7 +571,7 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
     // two stages at a time where a stage is an odd number of steps: the
     // fragment buffers are then compile-time
     constexpr int AT = SPS & 1 ? 2 : 1;
-    for (; s + AT - 1 + SLOTS < full; s += AT) {
+    for (; s + AT - 1 + SLOTS + (REG ? 1 : 0) < full; s += AT) {
 #pragma unroll
       for (int u = 0; u < AT; ++u) {
         stage(s + u, slot, after(slot), u * SPS & 1, true);
@@ -624,23 +674,23 @@ long row_tiles(const LinearArgs& a, int BM) {
   return t < a.M ? t : a.M;
 }
 
-template <bool F8, int WN, int WM, int NI, int MJ, int KB, int SLOTS, int WPE>
+template <bool F8, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE>
 hipError_t launch_tile(const LinearArgs& a, hipStream_t s) {
   constexpr int TN = 32 * WN * NI, TM = 32 * WM * MJ;
   const long nbn = (a.N + TN - 1) / TN, nbm = row_tiles(a, TM);
   if (!grid_fits(nbm * nbn, WN * WM * 64)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((linear_tile_kernel<F8, WN, WM, NI, MJ, KB, SLOTS, WPE>), dim3((unsigned)(nbm * nbn)),
+  hipLaunchKernelGGL((linear_tile_kernel<F8, REG, WN, WM, NI, MJ, NV, KB, SLOTS, WPE>), dim3((unsigned)(nbm * nbn)),
                      dim3(WN * WM * 64), 0, s, a, (int)nbm, (int)nbn);
   return hipGetLastError();
 }
 
-template <bool F8, int MI, int NJ, int WK, int U>
-hipError_t launch_direct(const LinearArgs& a, hipStream_t s) {
+template <bool F8, bool ODD, int MI, int NJ, int WK, int U>
+hipError_t launch_direct_as(const LinearArgs& a, hipStream_t s) {
   constexpr int BM = 16 * MI, BN = 16 * NJ;
   const long nbn = (a.N + BN - 1) / BN;
   const long mt = row_tiles(a, BM);
   if (!grid_fits(mt * nbn, WK * 64)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((linear_direct_kernel<F8, MI, NJ, WK, U>), dim3((unsigned)(mt * nbn)), dim3(WK * 64), 0, s, a,
+  hipLaunchKernelGGL((linear_direct_kernel<F8, ODD, MI, NJ, WK, U>), dim3((unsigned)(mt * nbn)), dim3(WK * 64), 0, s, a,
                      (int)mt);
   return hipGetLastError();
 }
@@ -667,7 +717,7 @@ int num_cus() {
 //   2048 x 4096 x 4096                          70 / 65   45 / 43    67 / 60
 //   4096 x 4096 x 4096                         129 / 118  84 / 81    74 / 68
 //   8192 x 8192 x 8192                         910 / 810 566 / 493  497 / 430
-// A tile's stage costs what its DMA and its chain of steps take, nearly the
+// A tile's stage costs what its loads and its chain of steps take, nearly the
 // same whatever else runs: so the tiles are compared by rounds of workgroups
 // times a round's cost per K (per 1024 of K, first with one workgroup per CU,
 // then with two).
@@ -675,7 +725,11 @@ struct TileCost {
   int tn, tm, per_cu;
   float one, two, fixed;
 };
-constexpr TileCost kTiles[3] = {{64, 64, 2, 2.9f, 4.4f, 3.f}, {128, 128, 2, 6.5f, 10.f, 4.f}, {256, 256, 1, 16.f, 16.f, 7.f}};
+constexpr int kTileKinds = 4;
+constexpr TileCost kTiles[kTileKinds] = {{64, 64, 2, 2.0f, 3.3f, 2.5f},     // 64 x 64, 5 slots
+                                         {128, 128, 1, 4.5f, 5.2f, 5.f},    // 128 x 128, 4 slots
+                                         {128, 128, 2, 5.0f, 9.0f, 4.f},    // 128 x 128, 2 slots
+                                         {256, 256, 1, 15.f, 15.f, 9.f}};   // 256 x 256, 2 slots
 
 // rows' tiles of height tm; grouped: as if each expert's last one were half full
 float tiles_of_rows(const LinearArgs& a, int tm) {
@@ -688,7 +742,7 @@ int best_tile(const LinearArgs& a) {
   int best = 0;
   float least = 0.f;
   const float cus = (float)num_cus();
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < kTileKinds; ++i) {
     const TileCost& t = kTiles[i];
     const float wgs = tiles_of_rows(a, t.tm) * (float)((a.N + t.tn - 1) / t.tn), round = cus * t.per_cu;
     const float rounds = __builtin_floorf(wgs / round), rest = wgs - rounds * round;
@@ -702,19 +756,42 @@ int best_tile(const LinearArgs& a) {
   return best;
 }
 
+template <bool F8, bool REG>
+hipError_t launch_best_tile(const LinearArgs& a, hipStream_t s) {
+  switch (best_tile(a)) {
+    case 0: return launch_tile<F8, REG, 2, 2, 1, 1, 4, 128, REG ? 3 : 5, 2>(a, s);
+    case 1:
+      if constexpr (!REG) return launch_tile<F8, REG, 2, 2, 2, 2, 4, 128, 4, 1>(a, s);
+      [[fallthrough]];
+    case 2: return launch_tile<F8, REG, 2, 2, 2, 2, 2, 128, 2, 2>(a, s);
+    default:
+      if constexpr (!REG) return launch_tile<F8, REG, 2, 2, 4, 4, 2, 128, 2, 1>(a, s);
+      return launch_tile<F8, REG, 2, 2, 2, 2, 2, 128, 2, 2>(a, s);
+  }
+}
+
+template <bool F8, int MI, int NJ, int WK, int U>
+hipError_t launch_direct(const LinearArgs& a, hipStream_t s) {
+  return a.odd ? launch_direct_as<F8, true, MI, NJ, WK, U>(a, s) : launch_direct_as<F8, false, MI, NJ, WK, U>(a, s);
+}
+
 template <bool F8>
 hipError_t launch_linear_any(const LinearArgs& a, bool dma, hipStream_t s) {
   const float rows = a.E ? (float)a.M / a.E : (float)a.M;  // rows that share weights
   const float wgs = tiles_of_rows(a, 64) * (float)((a.N + 63) / 64);
-  if (rows <= 16.f)
+  const float cus = (float)num_cus();
+  if (rows <= 16.f) {
+    // a slice of K per wave: more of them where K is long or workgroups are few
+    if (a.K >= 2048 && tiles_of_rows(a, 16) * (float)((a.N + 15) / 16) < 0.25f * cus)
+      return launch_direct<F8, 1, 1, 16, 4>(a, s);
     return a.K < 8192 ? launch_direct<F8, 1, 1, 4, 4>(a, s) : launch_direct<F8, 1, 1, 8, 4>(a, s);
-  // half the chip's CUs are not enough to pull the weights by 64 x 64 tiles
-  if (dma && (!F8 || a.bf16) && wgs >= 0.5f * num_cus()) switch (best_tile(a)) {
-      case 0: return launch_tile<F8, 2, 2, 1, 1, 128, 5, 2>(a, s);
-      case 1: return launch_tile<F8, 2, 2, 2, 2, 128, 2, 2>(a, s);
-      default: return launch_tile<F8, 2, 2, 4, 4, 128, 2, 1>(a, s);
-    }
-  if (wgs < (float)num_cus()) return launch_direct<F8, 2, 2, 4, 4>(a, s);
+  }
+  // a quarter of the CUs are not enough to pull the weights by 64 x 64 tiles
+  // (a tile's row offsets are 32 bits)
+  if ((!F8 || a.bf16) && wgs >= 0.25f * cus && a.ldx <= (1 << 22) && a.ldw <= (1 << 22))
+    return dma ? launch_best_tile<F8, false>(a, s) : launch_best_tile<F8, true>(a, s);
+  if (wgs < cus)
+    return a.K >= 2048 && wgs < 0.125f * cus ? launch_direct<F8, 2, 2, 16, 1>(a, s) : launch_direct<F8, 2, 2, 4, 4>(a, s);
   return launch_direct<F8, 4, 4, 4, 2>(a, s);
 }
 
@@ -754,10 +831,10 @@ int linear_any(const char* who, const dlq_linear_desc* d, int E, const int32_t* 
   a.bf16 = d->out_type == DLQ_T_BF16;
   a.vec = ((uintptr_t)ws | (uintptr_t)bias) % 16 == 0 && ((uintptr_t)y | (uintptr_t)res) % (4 * es) == 0 &&
           d->N % 4 == 0 && d->ldy % 4 == 0 && (!res || d->ldr % 4 == 0);
+  a.odd = ((uintptr_t)x | (uintptr_t)w | (uintptr_t)d->ldx | (uintptr_t)d->ldw) % 4 != 0;
   a.E = E;
   a.off = off;
-  const bool dma = ((uintptr_t)x | (uintptr_t)w) % 16 == 0 && d->K % 16 == 0 && d->ldx % 16 == 0 && d->ldw % 16 == 0 &&
-                   d->ldx <= (1 << 22) && d->ldw <= (1 << 22);  // a tile's offsets fit 32 bits
+  const bool dma = ((uintptr_t)x | (uintptr_t)w) % 16 == 0 && d->K % 16 == 0 && d->ldx % 16 == 0 && d->ldw % 16 == 0;
   const hipError_t e = launch_linear_any<F8>(a, dma, (hipStream_t)stream);
   return e == hipSuccess ? DLQ_OK : fail(DLQ_ERR_LAUNCH, std::string(who) + " launch: " + hipGetErrorString(e));
 }

@@ -17,8 +17,10 @@
 // largest of its 64 lane maxima; the smallest of these has at least `top`
 // logits at or above it, so only those -- one to two times `top` -- go to a
 // list in LDS, and an entry's place is the number of larger entries.  Where
-// equal values outgrow the list, the bound is taken again on value and index
-// together; a chunk with a NaN takes `top` rounds of a plain maximum.
+// that bound lets too many through (equal values, mostly masked rows) or a NaN
+// is about, the exact bound is found: the top-th largest value bit by bit,
+// counting over all logits of the chunk, then the index up to which the ones
+// equal to it count.
 #include "rowops_common.h"
 
 namespace dlq {
@@ -26,7 +28,7 @@ namespace {
 
 typedef unsigned long long u64;
 constexpr int kLane = 32;   // logits per lane
-constexpr int kList = 512;  // entries of a group's list
+constexpr int kList = 512;  // entries of the join's list
 constexpr float kNan = __builtin_nanf("");
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
@@ -165,10 +167,8 @@ __device__ __forceinline__ void place_entries(const u64* list, int n, int tid, i
   }
 }
 
-// A number that n of a wave's 64 keys reach and that is above the others, bit
-// by bit from above (EXACT: the nth largest key, which equal ones may reach
-// too); 0 if fewer than n keys are not 0.
-template <bool EXACT = false>
+// A number that n of a wave's 64 keys reach, no larger than the nth largest and
+// above the next smaller, bit by bit from above; 0 if fewer than n are not 0.
 __device__ __forceinline__ unsigned wave_nth(unsigned key, int n) {
   unsigned bound = 0;
 #pragma unroll 1
@@ -176,7 +176,7 @@ __device__ __forceinline__ unsigned wave_nth(unsigned key, int n) {
     const unsigned c = bound | 1u << b;
     const int reach = __popcll(__ballot(key >= c));
     if (reach >= n) bound = c;
-    if (!EXACT && reach == n) break;
+    if (reach == n) break;
   }
   return bound;
 }
@@ -185,8 +185,9 @@ template <bool BF16, int NW>
 __global__ __launch_bounds__(256) void logprobs_chunk_kernel(const LogprobArgs a, int rows) {
   constexpr int G = 4 / NW, TPG = 64 * NW, NL = kLane, CHUNK = TPG * NL;
   constexpr int EPV = BF16 ? 8 : 4, NV = NL / EPV;  // logits per 16-byte load, loads per lane
-  __shared__ u64 lists[G][kList];
-  __shared__ u64 kbuf[4];
+  // entries of a group's list: with more, placing them costs more than the exact bound
+  constexpr int kMany = NW == 1 ? 192 : 384;
+  __shared__ u64 lists[G][kMany];
   __shared__ Part pbuf[4];
   __shared__ unsigned ubuf[4];
   __shared__ int counts[G];
@@ -227,8 +228,11 @@ __global__ __launch_bounds__(256) void logprobs_chunk_kernel(const LogprobArgs a
       if (j + EPV <= left) {
         spread(v, *(const v4i_any*)(base + (size_t)(v * TPG + t) * 16));
       } else {
+        constexpr int SZ = BF16 ? 2 : 4;
+        spread(v, load_tail16<false>(base + (size_t)(v * TPG + t) * 16, (left - j) * SZ, chunk ? 16 : j * SZ));
 #pragma unroll
-        for (int i = 0; i < EPV; ++i) x[v * EPV + i] = j + i < left ? logit<BF16>(a.x, x0 + j + i) : -INFINITY;
+        for (int i = 0; i < EPV; ++i)
+          if (j + i >= left) x[v * EPV + i] = -INFINITY;
       }
     }
   }
@@ -312,13 +316,13 @@ __global__ __launch_bounds__(256) void logprobs_chunk_kernel(const LogprobArgs a
       out[k] = key;
   };
 
-  int n = 0;
+  int n = kMany + 1;
   if (!plain) {
     if (NW > 1 && bound == 0)  // a short last chunk leaves waves empty: one wave's top-th
       bound = group_join<NW>(wave_nth(key, a.top), ubuf, [](unsigned p, unsigned q) { return p > q ? p : q; });
     if (bound <= value_key(-INFINITY)) {
-      // few logits, or few that are not masked: all of them, if they fit
-      if (left <= kList) {
+      // few logits, or few that are not masked: all of them, if they are not too many
+      if (left <= kMany) {
 #pragma unroll
         for (int e = 0; e < NL; ++e) {
           const int j = (e / EPV * TPG + t) * EPV + e % EPV;
@@ -336,56 +340,73 @@ __global__ __launch_bounds__(256) void logprobs_chunk_kernel(const LogprobArgs a
             for (int e = 4 * q; e < 4 * q + 4; ++e)
               if (x[e] >= least) {
                 const int at = atomicAdd(&counts[g], 1);
-                if (at < kList) list[at] = entry_key(x[e], first + (e / EPV * TPG + t) * EPV + e % EPV);
+                if (at < kMany) list[at] = entry_key(x[e], first + (e / EPV * TPG + t) * EPV + e % EPV);
               }
           }
       }
     }
     group_sync<NW>();
     n = counts[g];
-    if (n > kList) {
-      // equal values: the top-th largest of one wave's lane maxima together
-      // with the (lowest) places where the lanes hold them
-      int place = 0;
+  }
+  if (n > kMany) {
+    // keys in place of the logits, 0 past K: how many of the chunk reach c
+    unsigned k[NL];
 #pragma unroll
-      for (int e = NL - 1; e >= 0; --e)
-        if (x[e] == mine) place = (e / EPV * TPG + t) * EPV + e % EPV;
-      const unsigned value = wave_nth<true>(key, a.top);
-      const int above = __popcll(__ballot(key > value));
-      const unsigned tie = wave_nth(key == value ? ~(unsigned)place : 0u, a.top - above);
-      const u64 both = group_join<NW>(value ? (u64)value << 32 | tie : 0, kbuf, [](u64 p, u64 q) { return p > q ? p : q; });
-      if (t == 0) counts[g] = 0;
-      group_sync<NW>();
+    for (int e = 0; e < NL; ++e) {
+      const int j = (e / EPV * TPG + t) * EPV + e % EPV;
+      k[e] = j < left ? value_key(x[e]) : 0u;
+    }
+    const auto total = [&](int mine) {  // over the group, from the waves' counts
+      if constexpr (NW > 1) mine = group_join<NW>(mine, (int*)ubuf, [](int p, int q) { return p + q; });
+      return mine;
+    };
+    unsigned value = 0;
+    int above = 0;  // keys above `value`
+    bool exact = false;
+#pragma unroll 1
+    for (int b = 31; b >= 0 && !exact; --b) {
+      const unsigned c = value | 1u << b;
+      int reach = 0;
 #pragma unroll
-      for (int e = 0; e < NL; ++e) {
-        const int j = (e / EPV * TPG + t) * EPV + e % EPV;
-        if (j < left && entry_key(x[e], j) >= both) {
-          const int at = atomicAdd(&counts[g], 1);
-          if (at < kList) list[at] = entry_key(x[e], first + j);
-        }
+      for (int e = 0; e < NL; ++e) reach += __popcll(__ballot(k[e] >= c));
+      reach = total(reach);
+      if (reach >= a.top)
+        value = c;
+      else
+        above = reach;
+      exact = reach == a.top;
+    }
+    // of the keys equal to `value`, those at the lowest top - above places
+    int place = CHUNK;  // all of them
+    if (!exact) {
+      place = 0;
+#pragma unroll 1
+      for (int b = CHUNK / 2; b > 0; b >>= 1) {
+        int before = 0;
+#pragma unroll
+        for (int e = 0; e < NL; ++e)
+          before += __popcll(__ballot(k[e] == value && (e / EPV * TPG + t) * EPV + e % EPV < place + b));
+        if (total(before) <= a.top - above) place += b;
       }
-      group_sync<NW>();
-      n = counts[g];
-      plain = n > kList;
     }
-  }
-  if (!plain) {
-    place_entries(list, n, t, TPG, a.top, put);
-    // a last chunk shorter than `top`: empty entries behind its own
-    for (int k = n + t; k < a.top; k += TPG) put(k, 0);
-    return;
-  }
-  u64 last = ~0ull;
-  const int here = left < CHUNK ? left : CHUNK;
-  for (int k = 0; k < a.top; ++k) {
-    u64 best = 0;
-    for (int j = t; j < here; j += TPG) {
-      const u64 c = entry_key(logit<BF16>(a.x, x0 + j), first + j);
-      if (c < last && c > best) best = c;
+    group_sync<NW>();
+    if (t == 0) counts[g] = 0;
+    group_sync<NW>();
+#pragma unroll
+    for (int e = 0; e < NL; ++e) {
+      const int j = (e / EPV * TPG + t) * EPV + e % EPV;
+      if (k[e] && (k[e] > value || (k[e] == value && j < place))) {
+        const int at = atomicAdd(&counts[g], 1);
+        if (at < kMany) list[at] = (u64)k[e] << 32 | (unsigned)~(first + j);
+      }
     }
-    last = group_join<NW>(wave_max(best), kbuf, [](u64 p, u64 q) { return p > q ? p : q; });
-    if (t == 0) put(k, last);
+    group_sync<NW>();
+    n = counts[g];
+    if (n > kMany) n = kMany;
   }
+  place_entries(list, n, t, TPG, a.top, put);
+  // a last chunk shorter than `top`: empty entries behind its own
+  for (int i = n + t; i < a.top; i += TPG) put(i, 0);
 }
 
 // The chunks of one row: a workgroup per row.

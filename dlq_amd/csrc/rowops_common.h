@@ -12,14 +12,62 @@ typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-// 16 bytes at any address: gfx950 takes unaligned vector memory accesses, so
-// this is one global_load_dwordx4 as well
 typedef v4i v4i_any __attribute__((aligned(1)));
 
-// 16 bytes of codes, those from `avail` on read as zero and not touched.
-__device__ __forceinline__ v4i load_codes16(const int8_t* p, int avail) {
-  if (avail >= 16) return *(const v4i_any*)p;
+// 16 bytes at any address: gfx950 takes them unaligned, but at a third of the
+// rate where they do not start on a dword (12 x 16 x 11178 int8, rows 2 bytes
+// off: 26.6 us, 8.8 on 8-byte rows).  ODD: the five dwords that hold them,
+// moved into place when they are used; the fifth, where there are only four,
+// is the fourth again, so that no dword is touched without a wanted byte in it.
+template <bool ODD>
+struct Raw16 {
+  v4i d;
+  __device__ __forceinline__ void load(const int8_t* p) { d = *(const v4i_any*)p; }
+  __device__ __forceinline__ v4i get(const int8_t*) const { return d; }
+};
+template <>
+struct Raw16<true> {
+  typedef v4i v4i_dword __attribute__((aligned(4)));
+  v4i d;
+  int e;
+  __device__ __forceinline__ void load(const int8_t* p) {
+    const uintptr_t at = (uintptr_t)p;
+    d = *(const v4i_dword*)(at & ~(uintptr_t)3);
+    e = *(const int*)((at + 15) & ~(uintptr_t)3);
+  }
+  // p: any address that lies as the loaded one does to a dword
+  __device__ __forceinline__ v4i get(const int8_t* p) const {
+    const unsigned o = (unsigned)(uintptr_t)p & 3;
+    return v4i{(int)__builtin_amdgcn_alignbyte((unsigned)d[1], (unsigned)d[0], o),
+               (int)__builtin_amdgcn_alignbyte((unsigned)d[2], (unsigned)d[1], o),
+               (int)__builtin_amdgcn_alignbyte((unsigned)d[3], (unsigned)d[2], o),
+               (int)__builtin_amdgcn_alignbyte((unsigned)e, (unsigned)d[3], o)};
+  }
+};
+
+// 16 bytes at p of which `avail` belong to the row, zeros in place of the
+// others, which are not touched.  before: bytes of the row in front of p; with
+// 16 up to the row's end the last 16 are loaded and moved down, one load
+// instead of a chain of bytes.
+template <bool ODD>
+__device__ __forceinline__ v4i load_tail16(const void* at, int avail, int before) {
+  const int8_t* p = (const int8_t*)at;
   v4i v = {0, 0, 0, 0};
+  if (avail <= 0) return v;
+  if (avail >= 16 || before + avail >= 16) {
+    const int less = avail >= 16 ? 0 : 16 - avail;
+    Raw16<ODD> r;
+    r.load(p - less);
+    v = r.get(p - less);
+    if (less) {
+      typedef unsigned long long u64;
+      const u64 lo = (u64)(unsigned)v[1] << 32 | (unsigned)v[0], hi = (u64)(unsigned)v[3] << 32 | (unsigned)v[2];
+      const int s = 8 * less;  // 8..120 bits
+      const u64 l = s < 64 ? lo >> s | hi << (64 - s) : hi >> (s - 64), h = s < 64 ? hi >> s : 0;
+      v = v4i{(int)l, (int)(l >> 32), (int)h, (int)(h >> 32)};
+    }
+    return v;
+  }
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     if (i < avail) v[i >> 2] |= (int)((unsigned)(uint8_t)p[i] << (8 * (i & 3)));

@@ -37,17 +37,10 @@ struct Vec {
   __device__ __forceinline__ void load(const void* x, size_t i) {
     r = *(const v4i_any*)((const char*)x + i * (BF16 ? 2 : 4));
   }
-  // the first `n` values, zeros behind them
-  __device__ __forceinline__ void load_part(const void* x, size_t i, int n) {
-    r = v4i{0, 0, 0, 0};
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if (k >= n) break;
-      if constexpr (BF16)
-        r[k >> 1] |= (int)((unsigned)((const uint16_t*)x)[i + k] << (16 * (k & 1)));
-      else
-        r[k] = ((const int*)x)[i + k];
-    }
+  // the last values of a row, from column c on; zeros behind them
+  __device__ __forceinline__ void load_end(const void* x, size_t x0, int c, int cols) {
+    constexpr int S = BF16 ? 2 : 4;
+    r = load_tail16<false>((const char*)x + (x0 + c) * S, (cols - c) * S < 16 ? (cols - c) * S : 16, c * S);
   }
   __device__ __forceinline__ unsigned most() const {
     unsigned u = 0;
@@ -95,7 +88,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_ker
     if (c + N <= cols)
       v[i].load(x, x0 + c);
     else if (c < cols)
-      v[i].load_part(x, x0 + c, cols - c);
+      v[i].load_end(x, x0, c, cols);
   }
   unsigned u = 0;
 #pragma unroll
@@ -106,7 +99,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_ker
     if (c + N <= cols)
       w.load(x, x0 + c);
     else
-      w.load_part(x, x0 + c, cols - c);
+      w.load_end(x, x0, c, cols);
     u = max(u, w.most());
   }
   u = (unsigned)wave_join((int)u, 0, [](int a, int b) { return (int)max((unsigned)a, (unsigned)b); });
@@ -145,7 +138,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_ker
     if (c + N <= cols)
       w.load(x, x0 + c);
     else
-      w.load_part(x, x0 + c, cols - c);
+      w.load_end(x, x0, c, cols);
     put(w, c);
   }
   for (int c = cols + t; c < ldq; c += TPR) qr[c] = 0;

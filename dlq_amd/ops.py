@@ -454,10 +454,16 @@ def block_l1_f8(x: torch.Tensor, w1: torch.Tensor, alpha1: torch.Tensor, beta1: 
 _TYPES = {torch.float32: DLQ_T_F32, torch.bfloat16: DLQ_T_BF16}
 
 
-def _rows(t: torch.Tensor, name: str, dtypes, rows=None, cols=None):
-    """Checks a row-strided CUDA matrix: its rows, columns and row stride in elements."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
+def _placed(t, name: str, dtypes, dev) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.get_device() < 0:
         raise TypeError(f"{name}: expected a CUDA tensor of {' or '.join(map(str, dtypes))}")
+    raise ValueError(f"{name}: on device {t.get_device()}, the first tensor is on {dev}")
+
+
+def _rows(t: torch.Tensor, name: str, dtypes, dev, rows=None, cols=None):
+    """Checks a row-strided CUDA matrix on device dev: its rows, columns and row stride in elements."""
+    if not (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.get_device() == dev >= 0):
+        _placed(t, name, dtypes, dev)
     shape = t.shape
     if len(shape) != 2 or (rows is not None and shape[0] != rows) or (cols is not None and shape[1] != cols):
         raise ValueError(f"{name}: shape {tuple(shape)}, expected [{'rows' if rows is None else rows}, "
@@ -471,37 +477,47 @@ def _rows(t: torch.Tensor, name: str, dtypes, rows=None, cols=None):
     return r, c, ld
 
 
-def _vector(t, name: str, dtype, shape):
-    """Checks an optional contiguous CUDA tensor; its address or None."""
+def _vector(t, name: str, dtypes, dev, shape):
+    """Checks an optional contiguous CUDA tensor on device dev; its address or None."""
     if t is None:
         return None
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.is_contiguous()):
-        raise TypeError(f"{name}: expected a contiguous CUDA tensor of {dtype}")
+    if not (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.get_device() == dev >= 0):
+        _placed(t, name, dtypes, dev)
     if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
     return t.data_ptr()
 
 
-def _launch(what: str, fn, tensors, *args) -> None:
-    """fn(*args, stream) on the tensors' one device and its current stream."""
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+def _device(x, name: str) -> int:
+    if not (isinstance(x, torch.Tensor) and x.is_cuda):
+        raise TypeError(f"{name}: expected a CUDA tensor")
+    return x.get_device()
+
+
+def _launch(what: str, fn, dev: int, *args) -> None:
+    """fn(*args, stream) on device dev and its current stream."""
     if dev == torch.cuda.current_device():
         rc = fn(*args, raw_stream(dev))
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, raw_stream(dev))
-    check(rc, what)
+    if rc:
+        check(rc, what)
+
+
+_F32, _I32 = (torch.float32,), (torch.int32,)
 
 
 def _quantize_rows_dyn(what, fn, dtype, x, ld):
-    rows, cols, ldx = _rows(x, "x", _TYPES)
-    q = x.new_empty((rows, cols if ld is None else ld), dtype=dtype)
+    dev = _device(x, "x")
+    rows, cols, ldx = _rows(x, "x", _TYPES, dev)
+    if ld is None:
+        ld = cols
+    q = x.new_empty((rows, ld), dtype=dtype)
     scale = x.new_empty(rows, dtype=torch.float32)
-    _launch(what, fn, (x,), x.data_ptr(), _TYPES[x.dtype], rows, cols, ldx, q.data_ptr(), cols if ld is None else ld,
-            scale.data_ptr())
+    _launch(what, fn, dev, x.data_ptr(), _TYPES[x.dtype], rows, cols, ldx, q.data_ptr(), ld, scale.data_ptr())
     return q, scale
 
 
@@ -518,44 +534,43 @@ def quantize_rows_dyn_f8(x: torch.Tensor, ld: int | None = None):
 
 
 def _linear(what, fn, code, x, w, x_scale, w_scale, bias, act, residual, out_dtype, out, offsets=None):
-    if act not in DLQ_ACT:
+    kind = DLQ_ACT.get(act)
+    if kind is None:
         raise ValueError(f"act must be one of {sorted(DLQ_ACT)}, got {act!r}")
     if out is not None:
         out_dtype = out.dtype
     if out_dtype not in _TYPES:
         raise TypeError("output must be torch.float32 or torch.bfloat16")
-    M, K, ldx = _rows(x, "x", (code,))
+    dev = _device(x, "x")
+    M, K, ldx = _rows(x, "x", (code,), dev)
     if offsets is None:
-        N, _, ldw = _rows(w, "w", (code,), cols=K)
+        N, _, ldw = _rows(w, "w", (code,), dev, cols=K)
         per_column = (N,)
     else:
-        if not (isinstance(w, torch.Tensor) and w.is_cuda and w.dtype == code and w.dim() == 3 and w.is_contiguous()):
-            raise TypeError(f"w: expected a contiguous CUDA tensor [E, N, K] of {code}")
+        if not isinstance(w, torch.Tensor) or w.dim() != 3 or w.shape[2] != K:
+            raise ValueError(f"w: expected a tensor [E, N, {K}]")
         E, N, ldw = w.shape
+        _vector(w, "w", (code,), dev, w.shape)
         per_column = (E, N)
-        if ldw != K:
-            raise ValueError(f"w: shape {tuple(w.shape)}, expected [E, N, {K}]")
     if w_scale is None:
         raise TypeError("w_scale is required")
-    sx = _vector(x_scale, "x_scale", torch.float32, (M,))
-    sw = _vector(w_scale, "w_scale", torch.float32, per_column)
-    sb = _vector(bias, "bias", torch.float32, per_column)
+    sx = _vector(x_scale, "x_scale", _F32, dev, (M,))
+    sw = _vector(w_scale, "w_scale", _F32, dev, per_column)
+    sb = _vector(bias, "bias", _F32, dev, per_column)
     res, ldr = None, 0
     if residual is not None:
-        ldr = _rows(residual, "residual", (out_dtype,), M, N)[2]
+        ldr = _rows(residual, "residual", (out_dtype,), dev, M, N)[2]
         res = residual.data_ptr()
     if out is None:
         out, ldy = x.new_empty((M, N), dtype=out_dtype), N
     else:
-        ldy = _rows(out, "out", (out_dtype,), M, N)[2]
-    d = C.byref(LinearDesc(M, N, K, ldx, ldw, ldy, ldr, DLQ_ACT[act], _TYPES[out_dtype]))
+        ldy = _rows(out, "out", _TYPES, dev, M, N)[2]
+    d = C.byref(LinearDesc(M, N, K, ldx, ldw, ldy, ldr, kind, _TYPES[out_dtype]))
     if offsets is None:
-        _launch(what, fn, (x, w, x_scale, w_scale, bias, residual, out), d, x.data_ptr(), sx, w.data_ptr(), sw, sb, res,
-                out.data_ptr())
+        _launch(what, fn, dev, d, x.data_ptr(), sx, w.data_ptr(), sw, sb, res, out.data_ptr())
     else:
-        at = _vector(offsets, "offsets", torch.int32, (E + 1,))
-        _launch(what, fn, (x, w, x_scale, w_scale, bias, residual, out, offsets), d, E, at, x.data_ptr(), sx,
-                w.data_ptr(), sw, sb, res, out.data_ptr())
+        at = _vector(offsets, "offsets", _I32, dev, (E + 1,))
+        _launch(what, fn, dev, d, E, at, x.data_ptr(), sx, w.data_ptr(), sw, sb, res, out.data_ptr())
     return out
 
 
@@ -615,14 +630,18 @@ def logprobs(x: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0) 
     """Log probabilities of fp32 / bf16 logits [rows, K] (dlq_logprobs): of
     tokens int32 [rows] (0 where negative), the rows' entropy, and the `top`
     (<= 64) largest with their indices, equal ones by ascending index."""
-    rows, K, ldx = _rows(x, "x", _TYPES)
-    t = _vector(tokens, "tokens", torch.int32, (rows,))
-    lp = None if tokens is None else x.new_empty(rows, dtype=torch.float32)
+    dev = _device(x, "x")
+    rows, K, ldx = _rows(x, "x", _TYPES, dev)
+    t = _vector(tokens, "tokens", _I32, dev, (rows,))
+    lp = None if t is None else x.new_empty(rows, dtype=torch.float32)
     ent = x.new_empty(rows, dtype=torch.float32)
-    ti = x.new_empty((rows, top), dtype=torch.int32) if top > 0 else None
-    tl = x.new_empty((rows, top), dtype=torch.float32) if top > 0 else None
+    ti = tl = ws = None
+    if top > 0:
+        ti = x.new_empty((rows, top), dtype=torch.int32)
+        tl = x.new_empty((rows, top), dtype=torch.float32)
     nb = lib.dlq_logprobs_workspace_bytes(rows, K, top)
-    ws = x.new_empty(nb, dtype=torch.uint8) if nb else None
-    _launch("logprobs", lib.dlq_logprobs, (x, tokens), x.data_ptr(), _TYPES[x.dtype], rows, K, ldx, t, top, ptr(lp),
+    if nb:
+        ws = x.new_empty(nb, dtype=torch.uint8)
+    _launch("logprobs", lib.dlq_logprobs, dev, x.data_ptr(), _TYPES[x.dtype], rows, K, ldx, t, top, ptr(lp),
             ent.data_ptr(), ptr(ti), ptr(tl), ptr(ws), nb)
     return LogProbs(lp, ent, ti, tl)
