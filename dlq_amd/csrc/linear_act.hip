@@ -441,26 +441,25 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
   };
   // piece r of stage st into a slot; whole: all of the stage lies within K.
   // REG (rows that are not 16-byte aligned, which the DMA cannot take): the
-  // piece of the stage before goes from registers into the slot, and the
-  // stage's own is loaded into them.
-  Raw16<true> held[REG ? PP : 1];  // pieces at the end of K: in place already
-  auto fetch = [&](int st, int r, bool whole) __attribute__((always_inline)) {
+  // stage goes from registers into the slot, and the stage after the next into
+  // the registers; hb: which of the two sets.
+  Raw16<true> held[REG ? 2 : 1][REG ? PP : 1];  // pieces at the end of K: in place already
+  auto fetch = [&](int st, int hb, int r, bool whole) __attribute__((always_inline)) {
     const int8_t* base = (r < PW ? wbase : xbase) + (size_t)st * KB;
     const unsigned v = r < PW ? vw[r < PW ? r : 0] : vx[r < PW ? 0 : r - PW];
-    if (whole || st < full) {
-      held[r].load(base + v);
-    } else {
-      held[r].d = load_tail16<true>(base + v, a.K - st * KB - 16 * chunk, st * KB + 16 * chunk);  // zeros past K
-    }
+    if (whole || st < full)
+      held[hb][r].load(base + v);
+    else
+      held[hb][r].d = load_tail16<true>(base + v, a.K - st * KB - 16 * chunk, st * KB + 16 * chunk);  // zeros past K
   };
-  auto stash = [&](int st, int slot, int r, bool whole) __attribute__((always_inline)) {
+  auto stash = [&](int st, int hb, int slot, int r, bool whole) __attribute__((always_inline)) {
     const int8_t* p = (r < PW ? wbase : xbase) + (r < PW ? vw[r < PW ? r : 0] : vx[r < PW ? 0 : r - PW]);
-    *(v4i*)(lds + slot_at(slot, r) + lane * 16) = whole || st < full ? held[r].get(p) : held[r].d;
+    *(v4i*)(lds + slot_at(slot, r) + lane * 16) = whole || st < full ? held[hb][r].get(p) : held[hb][r].d;
   };
-  auto issue = [&](int st, int slot, int r, bool whole) __attribute__((always_inline)) {
+  auto issue = [&](int st, int hb, int slot, int r, bool whole) __attribute__((always_inline)) {
     if constexpr (REG) {
-      stash(st, slot, r, whole);
-      fetch(st + 1, r, whole);
+      stash(st, hb, slot, r, whole);
+      fetch(st + 2, hb, r, whole);
       return;
     }
     const unsigned to = lds32 + slot_at(slot, r);
@@ -493,7 +492,7 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
   // one step's matrix instructions on buffer b; between them, in its first
   // half, the reads of the next step (rslot >= 0), and DMA pieces of stage dst
   // (dst >= 0)
-  auto step = [&](int b, int rslot, int rstep, int dst, int dslot, bool whole) __attribute__((always_inline)) {
+  auto step = [&](int b, int rslot, int rstep, int dst, int hb, int dslot, bool whole) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < NM; ++t) {
       const int i = t / MJ, j = t % MJ;
@@ -508,7 +507,7 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
       if (dst >= 0) {
 #pragma unroll
         for (int r = 0; r < PP; ++r)
-          if (r * NM / PP == t) issue(dst, dslot, r, whole);
+          if (r * NM / PP == t) issue(dst, hb, dslot, r, whole);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -516,9 +515,9 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
   // stage s, its first fragments in buffer b0; slot: where it lies, next: the
   // slot of s + 1.  Before its last step: stage s + 1 has landed everywhere,
   // and nobody reads stage s's slot any more, which stage s + SLOTS then takes.
-  auto stage = [&](int s, int slot, int next, int b0, bool whole) __attribute__((always_inline)) {
+  auto stage = [&](int s, int slot, int next, int b0, int hb, bool whole) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k + 1 < SPS; ++k) step((b0 + k) & 1, slot, k + 1, -1, 0, false);
+    for (int k = 0; k + 1 < SPS; ++k) step((b0 + k) & 1, slot, k + 1, -1, 0, 0, false);
     if (REG) {  // this wave's writes of stage s + 1 are done; its loads go on
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     } else if (whole) {
@@ -528,17 +527,24 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
     }
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    step((b0 + SPS - 1) & 1, next, 0, s + SLOTS, slot, whole);
+    step((b0 + SPS - 1) & 1, next, 0, s + SLOTS, hb, slot, whole);
+  };
+  auto last_stage = [&](int slot, int b0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k + 1 < SPS; ++k) step((b0 + k) & 1, slot, k + 1, -1, 0, 0, false);
+    step((b0 + SPS - 1) & 1, -1, 0, -1, 0, 0, false);
   };
 
   if constexpr (REG) {
 #pragma unroll
-    for (int r = 0; r < PP; ++r) fetch(0, r, false);
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int r = 0; r < PP; ++r) fetch(st, st, r, false);
   }
 #pragma unroll
   for (int st = 0; st < SLOTS; ++st)
 #pragma unroll
-    for (int r = 0; r < PP; ++r) issue(st, st, r, false);
+    for (int r = 0; r < PP; ++r) issue(st, st & 1, st, r, false);
   // the epilogue's operands, on their way before the sums begin
   constexpr int LPR = NI * 8, RPI = 64 / LPR, U = 4;  // lanes per row, rows per instruction, instructions in flight
   static_assert(32 % (RPI * U) == 0, "rows of a staging pass");
@@ -568,31 +574,28 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
     for (int q = 0; q < NR; ++q) read(0, 0, 0, q);
     int s = 0, slot = 0;
     const auto after = [](int k) { return k + 1 == SLOTS ? 0 : k + 1; };
-    // two stages at a time where a stage is an odd number of steps: the
-    // fragment buffers are then compile-time
-    constexpr int AT = SPS & 1 ? 2 : 1;
-    for (; s + AT - 1 + SLOTS + (REG ? 1 : 0) < full; s += AT) {
+    // two stages at a time where a stage is an odd number of steps or goes
+    // through registers: the buffers are then compile-time
+    constexpr int AT = SPS % 2 || REG ? 2 : 1;
+    for (; s + AT - 1 + SLOTS + (REG ? 2 : 0) < full; s += AT) {
 #pragma unroll
       for (int u = 0; u < AT; ++u) {
-        stage(s + u, slot, after(slot), u * SPS & 1, true);
+        stage(s + u, slot, after(slot), u * SPS & 1, (u + SLOTS) & 1, true);
         slot = after(slot);
       }
     }
     for (; s + AT < nst; s += AT) {
 #pragma unroll
       for (int u = 0; u < AT; ++u) {
-        stage(s + u, slot, after(slot), u * SPS & 1, false);
+        stage(s + u, slot, after(slot), u * SPS & 1, (u + SLOTS) & 1, false);
         slot = after(slot);
       }
     }
     if (AT == 2 && s + 1 < nst) {
-      stage(s, slot, after(slot), 0, false);
-      slot = after(slot);
-      step(1, -1, 0, -1, 0, false);
+      stage(s, slot, after(slot), 0, SLOTS & 1, false);
+      last_stage(after(slot), SPS & 1);
     } else {
-#pragma unroll
-      for (int k = 0; k + 1 < SPS; ++k) step(k & 1, slot, k + 1, -1, 0, false);
-      step((SPS - 1) & 1, -1, 0, -1, 0, false);
+      last_stage(slot, 0);
     }
   }
   __syncthreads();  // the slots become the epilogue's staging
@@ -706,30 +709,40 @@ int num_cus() {
   return n;
 }
 
-// Which kernel.  Measured on one box (us, weights from memory, s8 / e4m3):
-//   M x N x K           direct 16 / 32 / 64   64 x 64   128 x 128   256 x 256
-//   1 x 4096 x 4096      5.8 / 8.9 / 15          13        32
-//   16 x 4096 x 4096     6.8 / 10 / 16           13        32          62
-//   64 x 4096 x 4096      17 / 11 / 21           14        34
-//   256 x 4096 x 4096     59 / 32 / 21        14.8 / 13.6  34          67
-//   512 x 4096 x 4096    115 / 61 / 34        21.4 / 20.7  34          66
-//   1003 x 5000 x 2736   137 / 80 / 50          47 / 44    37        62 / 58
-//   2048 x 4096 x 4096                          70 / 65   45 / 43    67 / 60
-//   4096 x 4096 x 4096                         129 / 118  84 / 81    74 / 68
-//   8192 x 8192 x 8192                         910 / 810 566 / 493  497 / 430
+// Which kernel.  One box, us, weights from memory, 16-byte rows (int8; e4m3
+// within 10 %, 256 x 256 up to 15 % faster); then K odd, through registers.
+//                        direct            tiles
+//   M x N x K            16    32    64    64    128/4  128/2  256
+//   1 x 4096 x 4096     5.8   8.8    15    12     21     33     55
+//   16 x 4096 x 4096    6.8    10    16    12     21     33     55
+//   32 x 4096 x 4096     10    12    18    13     22     34     57
+//   32 x 12288 x 4096    26    21    20    16     24     35     58
+//   64 x 4096 x 4096     18    11    21    15     24     35     58
+//   256 x 4096 x 4096    59    33    21    14     26     35     62
+//   512 x 4096 x 4096   115    61    34    21     26     35     62
+//   1003 x 5000 x 2736  136    79    50    46     50     38     59
+//   2276 x 953 x 16128  471   258   177    83     77    112    194
+//   2048 x 4096 x 4096  450   232   125    70     54     42     62
+//   4096 x 4096 x 4096  897   455   241   127    106     83     69
+//   K odd:                                 64   128 x 64
+//   32 x 4096 x 4099     16    19    32    26
+//   64 x 4096 x 4099     27    18    39    29     39
+//   256 x 4096 x 4099    88    51    33    28     37
+//   1003 x 5000 x 2737  247   151   101    62     58
+//   4096 x 4096 x 4099 1316   721   483   229    174
 // A tile's stage costs what its loads and its chain of steps take, nearly the
 // same whatever else runs: so the tiles are compared by rounds of workgroups
-// times a round's cost per K (per 1024 of K, first with one workgroup per CU,
-// then with two).
+// times a round's cost (us per 1024 of K with one and with two workgroups on a
+// CU, and what a round costs besides).
 struct TileCost {
   int tn, tm, per_cu;
   float one, two, fixed;
 };
-constexpr int kTileKinds = 4;
-constexpr TileCost kTiles[kTileKinds] = {{64, 64, 2, 2.0f, 3.3f, 2.5f},     // 64 x 64, 5 slots
-                                         {128, 128, 1, 4.5f, 5.2f, 5.f},    // 128 x 128, 4 slots
-                                         {128, 128, 2, 5.0f, 9.0f, 4.f},    // 128 x 128, 2 slots
-                                         {256, 256, 1, 15.f, 15.f, 9.f}};   // 256 x 256, 2 slots
+constexpr TileCost kDmaTiles[4] = {{64, 64, 2, 2.0f, 3.3f, 2.5f},     // 64 x 64, 5 slots
+                                   {128, 128, 1, 4.5f, 5.2f, 5.f},    // 128 x 128, 4 slots
+                                   {128, 128, 2, 5.0f, 9.0f, 4.f},    // 128 x 128, 2 slots
+                                   {256, 256, 1, 15.f, 15.f, 9.f}};   // 256 x 256, 2 slots
+constexpr TileCost kRegTiles[2] = {{64, 64, 2, 5.6f, 7.0f, 4.f}, {128, 64, 2, 8.0f, 9.9f, 5.f}};
 
 // rows' tiles of height tm; grouped: as if each expert's last one were half full
 float tiles_of_rows(const LinearArgs& a, int tm) {
@@ -738,15 +751,15 @@ float tiles_of_rows(const LinearArgs& a, int tm) {
   return t < a.M ? t : (float)a.M;
 }
 
-int best_tile(const LinearArgs& a) {
+template <int N>
+int best_tile(const LinearArgs& a, const TileCost (&tiles)[N]) {
   int best = 0;
   float least = 0.f;
-  const float cus = (float)num_cus();
-  for (int i = 0; i < kTileKinds; ++i) {
-    const TileCost& t = kTiles[i];
+  const float cus = (float)num_cus(), k = a.K / 1024.f;
+  for (int i = 0; i < N; ++i) {
+    const TileCost& t = tiles[i];
     const float wgs = tiles_of_rows(a, t.tm) * (float)((a.N + t.tn - 1) / t.tn), round = cus * t.per_cu;
     const float rounds = __builtin_floorf(wgs / round), rest = wgs - rounds * round;
-    const float k = a.K / 1024.f;
     const float c = rounds * (t.two * k + t.fixed) + (rest <= 0.f ? 0.f : (rest <= cus ? t.one : t.two) * k + t.fixed);
     if (i == 0 || c < least) {
       least = c;
@@ -756,17 +769,17 @@ int best_tile(const LinearArgs& a) {
   return best;
 }
 
-template <bool F8, bool REG>
-hipError_t launch_best_tile(const LinearArgs& a, hipStream_t s) {
-  switch (best_tile(a)) {
-    case 0: return launch_tile<F8, REG, 2, 2, 1, 1, 4, 128, REG ? 3 : 5, 2>(a, s);
-    case 1:
-      if constexpr (!REG) return launch_tile<F8, REG, 2, 2, 2, 2, 4, 128, 4, 1>(a, s);
-      [[fallthrough]];
-    case 2: return launch_tile<F8, REG, 2, 2, 2, 2, 2, 128, 2, 2>(a, s);
-    default:
-      if constexpr (!REG) return launch_tile<F8, REG, 2, 2, 4, 4, 2, 128, 2, 1>(a, s);
-      return launch_tile<F8, REG, 2, 2, 2, 2, 2, 128, 2, 2>(a, s);
+template <bool F8>
+hipError_t launch_best_tile(const LinearArgs& a, bool dma, hipStream_t s) {
+  if (!dma) {
+    if (best_tile(a, kRegTiles) == 0) return launch_tile<F8, true, 2, 2, 1, 1, 4, 128, 2, 2>(a, s);
+    return launch_tile<F8, true, 2, 2, 2, 1, 2, 128, 2, 2>(a, s);
+  }
+  switch (best_tile(a, kDmaTiles)) {
+    case 0: return launch_tile<F8, false, 2, 2, 1, 1, 4, 128, 5, 2>(a, s);
+    case 1: return launch_tile<F8, false, 2, 2, 2, 2, 4, 128, 4, 1>(a, s);
+    case 2: return launch_tile<F8, false, 2, 2, 2, 2, 2, 128, 2, 2>(a, s);
+    default: return launch_tile<F8, false, 2, 2, 4, 4, 2, 128, 2, 1>(a, s);
   }
 }
 
@@ -778,21 +791,14 @@ hipError_t launch_direct(const LinearArgs& a, hipStream_t s) {
 template <bool F8>
 hipError_t launch_linear_any(const LinearArgs& a, bool dma, hipStream_t s) {
   const float rows = a.E ? (float)a.M / a.E : (float)a.M;  // rows that share weights
-  const float wgs = tiles_of_rows(a, 64) * (float)((a.N + 63) / 64);
   const float cus = (float)num_cus();
-  if (rows <= 16.f) {
-    // a slice of K per wave: more of them where K is long or workgroups are few
-    if (a.K >= 2048 && tiles_of_rows(a, 16) * (float)((a.N + 15) / 16) < 0.25f * cus)
-      return launch_direct<F8, 1, 1, 16, 4>(a, s);
+  const auto wgs = [&](int t) { return tiles_of_rows(a, t) * (float)((a.N + t - 1) / t); };
+  // tiles from half as many workgroups as CUs on; their row offsets are 32 bits
+  if (rows > 16.f && wgs(64) >= 0.5f * cus && (!F8 || a.bf16) && a.ldx <= (1 << 22) && a.ldw <= (1 << 22))
+    return launch_best_tile<F8>(a, dma, s);
+  if (rows <= 16.f || wgs(16) <= 2.f * cus)
     return a.K < 8192 ? launch_direct<F8, 1, 1, 4, 4>(a, s) : launch_direct<F8, 1, 1, 8, 4>(a, s);
-  }
-  // a quarter of the CUs are not enough to pull the weights by 64 x 64 tiles
-  // (a tile's row offsets are 32 bits)
-  if ((!F8 || a.bf16) && wgs >= 0.25f * cus && a.ldx <= (1 << 22) && a.ldw <= (1 << 22))
-    return dma ? launch_best_tile<F8, false>(a, s) : launch_best_tile<F8, true>(a, s);
-  if (wgs < cus)
-    return a.K >= 2048 && wgs < 0.125f * cus ? launch_direct<F8, 2, 2, 16, 1>(a, s) : launch_direct<F8, 2, 2, 4, 4>(a, s);
-  return launch_direct<F8, 4, 4, 4, 2>(a, s);
+  return wgs(64) < cus ? launch_direct<F8, 2, 2, 4, 4>(a, s) : launch_direct<F8, 4, 4, 4, 2>(a, s);
 }
 
 template <bool F8>
