@@ -738,10 +738,11 @@ struct TileCost {
   int tn, tm, per_cu;
   float one, two, fixed;
 };
-constexpr TileCost kDmaTiles[4] = {{64, 64, 2, 2.0f, 3.3f, 2.5f},     // 64 x 64, 5 slots
-                                   {128, 128, 1, 4.5f, 5.2f, 5.f},    // 128 x 128, 4 slots
-                                   {128, 128, 2, 5.0f, 9.0f, 4.f},    // 128 x 128, 2 slots
-                                   {256, 256, 1, 15.f, 15.f, 9.f}};   // 256 x 256, 2 slots
+template <bool F8>
+constexpr TileCost kDmaTiles[4] = {{64, 64, 2, 2.0f, 3.3f, 2.5f},   // 64 x 64, 5 slots
+                                   {128, 128, 1, 4.5f, 5.2f, 5.f},  // 128 x 128, 4 slots
+                                   {128, 128, 2, 5.0f, 9.0f, 4.f},  // 128 x 128, 2 slots
+                                   {256, 256, 1, F8 ? 13.5f : 15.f, F8 ? 13.5f : 15.f, 9.f}};  // 256 x 256, 2 slots
 constexpr TileCost kRegTiles[2] = {{64, 64, 2, 5.6f, 7.0f, 4.f}, {128, 64, 2, 8.0f, 9.9f, 5.f}};
 
 // rows' tiles of height tm; grouped: as if each expert's last one were half full
@@ -775,8 +776,8 @@ hipError_t launch_best_tile(const LinearArgs& a, bool dma, hipStream_t s) {
     if (best_tile(a, kRegTiles) == 0) return launch_tile<F8, true, 2, 2, 1, 1, 4, 128, 2, 2>(a, s);
     return launch_tile<F8, true, 2, 2, 2, 1, 2, 128, 2, 2>(a, s);
   }
-  switch (best_tile(a, kDmaTiles)) {
-    case 0: return launch_tile<F8, false, 2, 2, 1, 1, 4, 128, 5, 2>(a, s);
+  switch (best_tile(a, kDmaTiles<F8>)) {
+    case 0: return launch_tile<F8, false, 2, 2, 1, 1, F8 ? 2 : 4, 128, 5, 2>(a, s);
     case 1: return launch_tile<F8, false, 2, 2, 2, 2, 4, 128, 4, 1>(a, s);
     case 2: return launch_tile<F8, false, 2, 2, 2, 2, 2, 128, 2, 2>(a, s);
     default: return launch_tile<F8, false, 2, 2, 4, 4, 2, 128, 2, 1>(a, s);
