@@ -7,14 +7,13 @@ HIPCC ?= /opt/rocm/bin/hipcc
 ARCH ?= gfx950
 # -ffp-contract=off: the fp32 epilogue/host-prep op order is part of the
 # numerics contract (every fused multiply-add is an explicit fmaf).
-HIPFLAGS = --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-result
+# -packed-fp32-ops: no packed fp32 instructions (some of their forms have given
+# wrong results on this hardware); the host pass notes that it does not know it.
+HIPFLAGS = --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops
 SRC = dlq_amd/csrc/kernels.hip dlq_amd/csrc/conv3x3.hip dlq_amd/csrc/conv3x3i.hip dlq_amd/csrc/conv3x3s2i.hip dlq_amd/csrc/block_l1.hip dlq_amd/csrc/stem.hip dlq_amd/csrc/head.hip dlq_amd/csrc/layerops.hip dlq_amd/csrc/gemm.hip dlq_amd/csrc/preproc.hip dlq_amd/csrc/fp8.hip dlq_amd/csrc/ref_f32.hip dlq_amd/csrc/rowquant.hip dlq_amd/csrc/linear_act.hip dlq_amd/csrc/logprobs.hip dlq_amd/csrc/capi.cpp dlq_amd/csrc/resnet18.cpp dlq_amd/csrc/mlp.cpp dlq_amd/csrc/wpack.cpp
 HDR = include/dlq.h dlq_amd/csrc/dlq_internal.h dlq_amd/csrc/device_common.h dlq_amd/csrc/rowops_common.h
 
 all: dlq_amd/libdlq.so bin/dlq_e2e bin/dlq_step tools/check/libplancap.so oracle
-
-# the row operators' float code stays off the packed fp32 instructions
-build/rowquant.o build/linear_act.o build/logprobs.o: HIPFLAGS += -Xclang -target-feature -Xclang -packed-fp32-ops
 
 # the layer1 block interleaves its epilogue FMAs with MFMAs, and the convs'
 # epilogues run beside the partner waves' MFMAs: keep their FMAs scalar

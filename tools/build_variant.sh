@@ -14,7 +14,7 @@ FLAGS="$*"
 OUT=abvar/$NAME
 OBJ=scratch/abobj/$NAME
 mkdir -p $OUT $OBJ
-HIPFLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-result $FLAGS"
+HIPFLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops $FLAGS"
 pids=()
 objs=()
 SRC=${SRC:-dlq_amd/csrc}
