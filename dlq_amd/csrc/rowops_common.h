@@ -101,6 +101,36 @@ __device__ __forceinline__ int wave_join(int v, int none, F f) {
   return __builtin_amdgcn_readlane(v, 63);
 }
 
+// The same for floats, one instruction a step: lanes without a source keep what
+// they have.  A step reads what the last one wrote after two wait states, the
+// lane read after one.
+#define DLQ_DPP_STEP(op, ctrl) "s_nop 1\n\t" op " %0, %0, %0 " ctrl " bank_mask:0xf\n\t"
+#define DLQ_DPP_QUADS(op) DLQ_DPP_STEP(op, "row_shr:1 row_mask:0xf") DLQ_DPP_STEP(op, "row_shr:2 row_mask:0xf")
+#define DLQ_DPP_REST(op)                                                                              \
+  DLQ_DPP_STEP(op, "row_shr:4 row_mask:0xf")                                                          \
+  DLQ_DPP_STEP(op, "row_shr:8 row_mask:0xf")                                                          \
+  DLQ_DPP_STEP(op, "row_bcast:15 row_mask:0xa") DLQ_DPP_STEP(op, "row_bcast:31 row_mask:0xc") "s_nop 1"
+__device__ __forceinline__ float lane63(float v) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  asm(DLQ_DPP_QUADS("v_add_f32_dpp") DLQ_DPP_REST("v_add_f32_dpp") : "+v"(v));
+  return lane63(v);
+}
+// Lane 4 i + 3: the largest of lanes 4 i to 4 i + 3 (a NaN is never one).
+__device__ __forceinline__ float quad_max(float v) {
+  asm(DLQ_DPP_QUADS("v_max_f32_dpp") "s_nop 1" : "+v"(v));
+  return v;
+}
+__device__ __forceinline__ float wave_max_of_quads(float v) {
+  asm(DLQ_DPP_REST("v_max_f32_dpp") : "+v"(v));
+  return lane63(v);
+}
+__device__ __forceinline__ float wave_max(float v) { return wave_max_of_quads(quad_max(v)); }
+#undef DLQ_DPP_STEP
+#undef DLQ_DPP_QUADS
+#undef DLQ_DPP_REST
+
 // A launch's blocks * threads must stay below 2^32 (the dispatch packet's grid
 // size is 32 bits of work-items).
 inline bool grid_fits(long long blocks, int threads) { return blocks * threads < (1LL << 32); }

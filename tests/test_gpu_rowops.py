@@ -281,6 +281,29 @@ def test_grouped_offsets_outside(gpu):
     assert (buf[:4] == 3.0).all() and (buf[4 + T:] == 3.0).all()
 
 
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("T", [5, 900])
+def test_grouped_without_rows_or_products(gpu, t, T):
+    """Experts that all are empty leave everything as it was; no expert at all
+    too; K = 0 is the activated bias."""
+    rng = np.random.default_rng(T)
+    N = 720
+    c = grouped_case(rng, t, 4, T, N, 64, torch.bfloat16)
+    y = torch.full((T, N), 3.0, dtype=torch.bfloat16, device="cuda")
+    f = linear(t)[1]
+    for off in ([0] * 5, [T] * 5, [T // 2] * 5):
+        f(dev(c["x"]), torch.tensor(off, dtype=torch.int32, device="cuda"), dev(c["w"]), dev(c["xs"]), dev(c["ws"]),
+          dev(c["bias"]), out=y)
+    f(dev(c["x"]), torch.zeros(1, dtype=torch.int32, device="cuda"), dev(c["w"])[:0], dev(c["xs"]), dev(c["ws"])[:0],
+      dev(c["bias"])[:0], out=y)
+    assert (y == 3.0).all()
+    off = [0, T // 3, T // 3, T - 1, T]
+    c0 = {**c, "x": c["x"][:, :0], "w": c["w"][..., :0]}
+    f(dev(c0["x"]), torch.tensor(off, dtype=torch.int32, device="cuda"), dev(c0["w"]), dev(c["xs"]), dev(c["ws"]),
+      dev(c["bias"]), "silu", dev(c["res"]), out=y)
+    close(y, *grouped_reference(c0, off, t, "silu", torch.bfloat16, T))
+
+
 # ------------------------------------------------------------- quantisation
 
 def quant_reference(x, t, ld):
@@ -438,6 +461,35 @@ def test_logprobs_masked_and_tied(gpu, K, top):
     tokens = torch.tensor([0, K // 2, 5, K - 1, 0, 1, 3, 1, 2, K - 1, 0, K - 1], dtype=torch.int32)
     r = check_logprobs(x, tokens, top)
     assert r.entropy[0] == 0 and r.entropy[1] == 0 and torch.isneginf(r.logprob[0])
+
+
+@pytest.mark.parametrize("xt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("K,top", [(512, 33), (513, 17), (2048, 16), (4096, 64), (4097, 3), (8192, 20), (8200, 64),
+                                   (16385, 5), (131073, 64), (300007, 20)])
+def test_logprobs_ties_at_the_borders(gpu, xt, K, top):
+    """Equal values on both sides of where a row is split, in every mixture of
+    few and many, at both ends."""
+    rng = np.random.default_rng([K, top])
+    low = torch.finfo(xt).min
+    x = torch.from_numpy(rng.standard_normal((9, K)).astype(np.float32))
+    x[0] = x[0].round()                     # few levels
+    x[1] = (torch.arange(K) % 3).float()    # a third of the row on top
+    x[2, :] = -5.0
+    x[2, K // 2:] = 3.0                     # the ties lie in the second half
+    x[3, :] = low
+    x[3, -3:] = torch.tensor([1.0, 2.0, 1.0])[-min(3, K):]
+    x[4, : K - 70] = -math.inf              # about `top` left, at the end
+    x[5, 70:] = -math.inf
+    x[6] = 1.0
+    x[6, ::97] = 1.5                        # every group has the same largest
+    x[7] = torch.arange(K) // 7             # ascending in steps
+    x[8] = math.inf
+    x = x.to(xt)
+    r = check_logprobs(x[:8], torch.full((8,), K - 1, dtype=torch.int32), top, x.cuda()[:8])
+    assert r.top_idx[6, 0] == 0
+    from dlq_amd import ops
+    x[8, 5], x[8, K - 1] = math.nan, math.nan
+    assert np.array_equal(ops.logprobs(x[8:].cuda(), None, top).top_idx.cpu().numpy(), alternatives(x[8:], top))
 
 
 @pytest.mark.parametrize("K", [40, 5000, 30000])
