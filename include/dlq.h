@@ -566,7 +566,8 @@ int dlq_linear_act_f8(const dlq_linear_desc* d, const uint8_t* x, const float* x
  * bias[E][N]).  offsets[E+1] lies on the device (non-decreasing, within 0..M;
  * others are clamped into that range, never read or written beyond it).  Rows
  * of y before offsets[0] and from offsets[E] on are left as they were; experts
- * without a row cost nothing.  d->M: rows of x and y.  E <= 65535. */
+ * without a row cost next to nothing: their weights are not read.  d->M: rows
+ * of x and y.  E <= 65535. */
 int dlq_linear_grouped_s8(const dlq_linear_desc* d, int E, const int32_t* offsets, const int8_t* x,
                           const float* x_scale, const int8_t* w, const float* w_scale, const float* bias,
                           const void* residual, void* y, void* stream);
