@@ -332,7 +332,7 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
 
 // ---- large products: tiles through LDS ------------------------------------
 // TN columns (rows of w) by TM rows of x per workgroup of WN x WM waves, each
-// wave NI x MJ tiles of 32 x 32.  Both operands stream by LDS-DMA, 128 bytes
+// wave NI x MJ tiles of 32 x 32; RES: with a residual that vec allows.  Both operands stream by LDS-DMA, 128 bytes
 // of K per stage into SLOTS slots; row r of a slot is 128 bytes, its 16-byte
 // chunk c at 16 (c ^ ((r >> 1) & 7)), so the 16 rows a ds_read_b128 lane group
 // reads fall on 16 distinct bank quads (the DMA lanes fetch in that order;
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
 // Waves own 128 x 128 outputs where there are enough rows and columns: an LDS
 // byte then feeds 64 multiply-adds, and reads and DMA writes take 192 KB of
 // the 256 KB that LDS moves in a stage's 2048 matrix cycles (with 128 x 64
-// per wave: 256 KB, the bound).  8192^3, bf16 out: int8 506 us, 2.17 POPS, the
+// per wave: 256 KB, the bound).  8192^3, bf16 out: int8 495 us, 2.22 POPS, the
 // clock at 1.7 GHz by the power limit and the matrix unit busy 55 % of the
 // cycles; e4m3 440 us, 2.5 PFLOP/s.  Waves of 64 x 64 (128 x 128 tiles) read
 // LDS for as long as they multiply: 576 us.  The small tiles are bound by what
@@ -393,7 +393,7 @@ __device__ __forceinline__ const int8_t* uniform(const int8_t* p) {
   return (const int8_t*)((unsigned long long)hi << 32 | lo);
 }
 
-template <bool F8, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE>
+template <bool F8, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE, bool RES>
 __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const LinearArgs a, int nbm, int nbn) {
   typedef TileMma<F8, NV> MM;
   typedef typename MM::acc_t acc_t;
@@ -408,8 +408,11 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
   static_assert(NW % 2 == 0 && TN % (RPP * NW) == 0 && TM % (RPP * NW) == 0, "pieces per wave");
   static_assert(PP * (SLOTS - 1) <= 63, "counted waits");
   constexpr int PITCH = NI * 32 * 4 + 16;  // epilogue staging: 32 rows of a wave's columns
-  static_assert(NW * 32 * PITCH <= SLOTS * SLOT, "epilogue staging");
-  __shared__ __attribute__((aligned(16))) int8_t lds[SLOTS * SLOT];
+  // lanes per row, rows per instruction, instructions per 32 rows, in flight of the epilogue
+  constexpr int LPR = NI * 8, RPI = 64 / LPR, NP = 32 / RPI, U = 4;
+  static_assert(NP % U == 0, "rows of a staging pass");
+  constexpr int EPILOGUE = NW * (32 * PITCH + (RES ? NP * 1024 : 0));  // staging, residual
+  __shared__ __attribute__((aligned(16))) int8_t lds[SLOTS * SLOT > EPILOGUE ? SLOTS * SLOT : EPILOGUE];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, lh = lane >> 5, wn = wave % WN, wm = wave / WN;
@@ -558,8 +561,6 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
 #pragma unroll
     for (int r = 0; r < PP; ++r) issue(st, st & 1, st, r, false);
   // the epilogue's operands, on their way before the sums begin
-  constexpr int LPR = NI * 8, RPI = 64 / LPR, U = 4;  // lanes per row, rows per instruction, instructions in flight
-  static_assert(32 % (RPI * U) == 0, "rows of a staging pass");
   const int cn = n0 + wn * NI * 32 + 4 * (lane % LPR), cr = lane / LPR;
   const bool in = cn < a.N;
   v4f ws = {0.f, 0.f, 0.f, 0.f}, bias = ws;
@@ -618,7 +619,57 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
   // is a real one (only the accumulator reads are per j): unrolled, with five
   // activations, the epilogue outgrew the instruction cache and cost as much
   // as 4096 of K.
+  // A residual's loads (bf16: three j ahead; fp32: one) go in front
+  // of the stores they would otherwise wait behind, and lie in LDS for the lane
+  // that loaded them; rows and columns that do not exist repeat one that does.
+  // 4096^3 int8 with a bf16 residual 73 us (loaded where it is added: 89; with
+  // none 72), 8192 x 8192 x 2048 179 (243; 151).  Its own kernel: as a branch
+  // of one, it cost products without a residual 2 us a round.
   int8_t* mine = lds + wave * 32 * PITCH;
+  v4f* held_res = (v4f*)(lds + NW * 32 * PITCH + wave * NP * 1024) + lane;
+  // bf16: j's in rw[j mod SB]; fp32: its halves in rw[0] and rw[1]
+  constexpr int SB = MJ > 3 ? 3 : MJ;
+  v2u rw[SB > 2 ? SB : 2][NP];
+  const char* rbase = (const char*)uniform((const int8_t*)a.res + ((size_t)m0 * a.ldr) * (a.bf16 ? 2 : 4));
+  const unsigned ldr = (unsigned)a.ldr * (a.bf16 ? 2 : 4), rcol = (unsigned)(in ? cn : 0) * (a.bf16 ? 2 : 4);
+  const auto residual_at = [&](int j, int i) __attribute__((always_inline)) {
+    int m = cr;
+    asm volatile("" : "+v"(m));  // the addresses are made here, not all in front of the loop
+    m += (wm * MJ + j) * 32 + i * RPI;
+    const int last = m1 - 1 - m0;
+    return rbase + ((unsigned)(m < last ? m : last) * ldr + rcol);
+  };
+  const auto fetch_bf16 = [&](auto jc) __attribute__((always_inline)) {
+    constexpr int j = decltype(jc)::value;
+    if constexpr (j < MJ) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        rw[j % SB][i] = *(const v2u*)residual_at(j, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  const auto fetch_f32 = [&](auto jc) __attribute__((always_inline)) {
+    constexpr int j = decltype(jc)::value;
+    if constexpr (j < MJ) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const v4u v = *(const v4u*)residual_at(j, i);
+        rw[0][i] = v2u{v[0], v[1]};
+        rw[1][i] = v2u{v[2], v[3]};
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  if (RES) {
+    if (a.bf16) {
+      fetch_bf16(std::integral_constant<int, 0>{});
+      if constexpr (SB > 1) fetch_bf16(std::integral_constant<int, 1>{});
+      if constexpr (SB > 2) fetch_bf16(std::integral_constant<int, 2>{});
+    } else {
+      fetch_f32(std::integral_constant<int, 0>{});
+    }
+  }
   auto stage_out = [&](auto jc) __attribute__((always_inline)) {
     constexpr int j = decltype(jc)::value;
 #pragma unroll
@@ -628,6 +679,21 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
         *(sum4*)(mine + lr * PITCH + (i * 32 + 8 * q + 4 * lh) * 4) =
             sum4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
     if (lh == 0) *(float*)(mine + lr * PITCH + NI * 128) = sxr[j];
+    if constexpr (RES) {
+      if (a.bf16) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const v2u h = rw[j % SB][i];
+          held_res[i * 64] = v4f{bf_lo(h[0]), bf_hi(h[0]), bf_lo(h[1]), bf_hi(h[1])};
+        }
+        fetch_bf16(std::integral_constant<int, j + SB>{});
+      } else {
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          *(v4u*)&held_res[i * 64] = v4u{rw[0][i][0], rw[0][i][1], rw[1][i][0], rw[1][i][1]};
+        fetch_f32(std::integral_constant<int, j + 1>{});
+      }
+    }
   };
 #pragma unroll 1
   for (int j = 0; j < MJ; ++j) {
@@ -641,38 +707,31 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
     asm volatile("" ::: "memory");
     const int mj = m0 + (wm * MJ + j) * 32 + cr;
 #pragma unroll 1
-    for (int t = 0; t < 32; t += RPI * U) {
+    for (int i = 0; i < NP; i += U) {
       v4f v[U], r[U];
       float sx[U];
-      if (a.vec && a.res) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int m = mj + t + u * RPI;
-          r[u] = v4f{0.f, 0.f, 0.f, 0.f};
-          if (m < m1 && in) r[u] = residual4(a, m, cn);
-        }
-      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int8_t* p = mine + (t + u * RPI + cr) * PITCH;
+        const int8_t* p = mine + ((i + u) * RPI + cr) * PITCH;
         const sum4 c = *(const sum4*)(p + 16 * (lane % LPR));
         v[u] = v4f{(float)c[0], (float)c[1], (float)c[2], (float)c[3]};
         sx[u] = *(const float*)(p + NI * 128);
+        if (RES) r[u] = held_res[(i + u) * 64];
       }
       with_act(a.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = scaled4<decltype(act)::value>(v[u], sx[u], ws, bias);
       });
-      if (a.vec) {
+      if (RES || a.vec) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int m = mj + t + u * RPI;
-          if (m < m1 && in) put4(a, m, cn, a.res ? v[u] + r[u] : v[u]);
+          const int m = mj + (i + u) * RPI;
+          if (m < m1 && in) put4(a, m, cn, RES ? v[u] + r[u] : v[u]);
         }
       } else {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int m = mj + t + u * RPI;
+          const int m = mj + (i + u) * RPI;
           if (m < m1 && in) put4_any(a, m, cn, v[u]);
         }
       }
@@ -694,8 +753,13 @@ hipError_t launch_tile(const LinearArgs& a, hipStream_t s) {
   constexpr int TN = 32 * WN * NI, TM = 32 * WM * MJ;
   const long nbn = (a.N + TN - 1) / TN, nbm = row_tiles(a, TM);
   if (!grid_fits(nbm * nbn, WN * WM * 64)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((linear_tile_kernel<F8, REG, WN, WM, NI, MJ, NV, KB, SLOTS, WPE>), dim3((unsigned)(nbm * nbn)),
-                     dim3(WN * WM * 64), 0, s, a, (int)nbm, (int)nbn);
+  const dim3 grid((unsigned)(nbm * nbn)), threads(WN * WM * 64);
+  if (a.vec && a.res)
+    hipLaunchKernelGGL((linear_tile_kernel<F8, REG, WN, WM, NI, MJ, NV, KB, SLOTS, WPE, true>), grid, threads, 0, s, a,
+                       (int)nbm, (int)nbn);
+  else
+    hipLaunchKernelGGL((linear_tile_kernel<F8, REG, WN, WM, NI, MJ, NV, KB, SLOTS, WPE, false>), grid, threads, 0, s, a,
+                       (int)nbm, (int)nbn);
   return hipGetLastError();
 }
 
@@ -806,8 +870,9 @@ hipError_t launch_linear_any(const LinearArgs& a, bool dma, hipStream_t s) {
   const float rows = a.E ? (float)a.M / a.E : (float)a.M;  // rows that share weights
   const float cus = (float)num_cus();
   const auto wgs = [&](int t) { return tiles_of_rows(a, t) * (float)((a.N + t - 1) / t); };
-  // tiles from half as many workgroups as CUs on; their row offsets are 32 bits
-  if (rows > 16.f && wgs(64) >= 0.5f * cus && (!F8 || a.bf16) && a.ldx <= (1 << 22) && a.ldw <= (1 << 22))
+  // tiles from half as many workgroups as CUs on; their rows' byte offsets are 32 bits
+  if (rows > 16.f && wgs(64) >= 0.5f * cus && (!F8 || a.bf16) && a.ldx <= (1 << 22) && a.ldw <= (1 << 22) &&
+      a.ldr <= (1 << 21))
     return launch_best_tile<F8>(a, dma, s);
   if (rows <= 16.f || wgs(16) <= 2.f * cus)
     return a.K < 8192 ? launch_direct<F8, 1, 1, 4, 4>(a, s) : launch_direct<F8, 1, 1, 8, 4>(a, s);

@@ -212,6 +212,22 @@ def test_linear_offsets_past_32_bits(gpu, t):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("M,N,ldr", [(300, 1700, 1 << 21), (300, 1700, (1 << 21) + 4), (700, 1028, 1028), (700, 1028, 1029)])
+def test_linear_residual_rows_far_apart(gpu, out, M, N, ldr):
+    """A residual whose rows lie further apart than a tile's 32-bit offsets
+    reach, up to there, and off 4 elements."""
+    rng = np.random.default_rng([M, ldr])
+    c = case(rng, "s8", M, N, 192, out)
+    big = torch.empty((M - 1) * ldr + N, dtype=out, device="cuda")
+    res = big.as_strided((M, N), (ldr, 1))
+    res.copy_(c["res"])
+    y = linear("s8")[0](dev(c["x"]), dev(c["w"]), dev(c["xs"]), dev(c["ws"]), dev(c["bias"]), "relu", res, out_dtype=out)
+    close(y, *product64(**c, act="relu", out_dtype=out))
+    del big, res
+    torch.cuda.empty_cache()
+
+
 def grouped_reference(c, off, t, act, out, T):
     y = torch.full((T, c["w"].shape[1]), 3.0, dtype=torch.float64)
     tol = torch.zeros_like(y)
