@@ -71,11 +71,15 @@ __device__ __forceinline__ void with_act(int act, F f) {
 
 // The residual's / the output's columns n..n+3 of row m, all of them below N
 // and aligned (a.vec).
-__device__ __forceinline__ v4f residual4(const LinearArgs& a, int m, int n) {
+__device__ __forceinline__ v4i residual_raw(const LinearArgs& a, int m, int n) {
   const size_t at = (size_t)m * a.ldr + n;
-  if (!a.bf16) return *(const v4f*)((const float*)a.res + at);
+  if (!a.bf16) return *(const v4i*)((const float*)a.res + at);
   const v2u r = *(const v2u*)((const uint16_t*)a.res + at);
-  return v4f{bf_lo(r[0]), bf_hi(r[0]), bf_lo(r[1]), bf_hi(r[1])};
+  return v4i{(int)r[0], (int)r[1], 0, 0};
+}
+__device__ __forceinline__ v4f residual_value(const LinearArgs& a, v4i r) {
+  if (!a.bf16) return v4f{__int_as_float(r[0]), __int_as_float(r[1]), __int_as_float(r[2]), __int_as_float(r[3])};
+  return v4f{bf_lo((unsigned)r[0]), bf_hi((unsigned)r[0]), bf_lo((unsigned)r[1]), bf_hi((unsigned)r[1])};
 }
 __device__ __forceinline__ void put4(const LinearArgs& a, int m, int n, v4f v) {
   const size_t at = (size_t)m * a.ldy + n;
@@ -207,7 +211,9 @@ struct Mma<true> {
 //
 // Bound by the weights' bytes, which a few rows read once, and below some
 // 20 MB by the latency of the loads: so each wave has 2 U of them in flight
-// (U steps ahead) and K is split until every CU has a workgroup.  int8, bf16
+// (U steps ahead), what is left of a slice is loaded at once (8 x 1000 x 2000
+// 3.4 us; step by step 4.5), so are the epilogue's operands, behind the first
+// loads, and K is split until every CU has a workgroup.  int8, bf16
 // out: 1 x 4096 x 4096 5.8 us (16.8 MB), 64 rows over 64 experts of
 // 1536 x 2048 24 us (about 40 of them have rows: 126 MB, 5.2 TB/s).
 template <bool F8, bool ODD, int MI, int NJ, int WK, int U>
@@ -245,14 +251,15 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
   const int s0 = (int)((long)steps * wave / WK), s1 = (int)((long)steps * (wave + 1) / WK);
   // U steps' loads are on their way while U others are multiplied
   Raw16<ODD> rx[2][U][MI], rw[2][U][NJ];
+  auto load_step = [&](int b, int u, int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) rw[b][u][j].load(wp[j] + (size_t)s * KB);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) rx[b][u][i].load(xp[i] + (size_t)s * KB);
+  };
   auto load = [&](int b, int s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) rw[b][u][j].load(wp[j] + (size_t)(s + u) * KB);
-#pragma unroll
-      for (int i = 0; i < MI; ++i) rx[b][u][i].load(xp[i] + (size_t)(s + u) * KB);
-    }
+    for (int u = 0; u < U; ++u) load_step(b, u, s + u);
   };
   auto product = [&](const v4i* vx, const v4i* vw) __attribute__((always_inline)) {
     typename MM::frag fx[MI], fw[NJ];
@@ -265,20 +272,42 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[i][j] = MM::go(fw[j], fx[i], acc[i][j]);
   };
+  auto multiply_step = [&](int b, int u) __attribute__((always_inline)) {
+    v4i vx[MI], vw[NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) vx[i] = rx[b][u][i].get(xp[i]);  // a step is a multiple of a dword
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) vw[j] = rw[b][u][j].get(wp[j]);
+    product(vx, vw);
+  };
   auto multiply = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      v4i vx[MI], vw[NJ];
-#pragma unroll
-      for (int i = 0; i < MI; ++i) vx[i] = rx[b][u][i].get(xp[i]);  // a step is a multiple of a dword
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) vw[j] = rw[b][u][j].get(wp[j]);
-      product(vx, vw);
-    }
+    for (int u = 0; u < U; ++u) multiply_step(b, u);
   };
+  // the epilogue's operands of one 16 x 16, on their way behind the first loads
+  // where a wave has no more than one
+  struct Ends {
+    float sx;
+    v4f ws, bias;
+    v4i res;
+  };
+  const auto ends = [&](int t) __attribute__((always_inline)) {
+    Ends o = {1.f, {0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}, {0, 0, 0, 0}};
+    const int m = m0 + 16 * (t / NJ) + lr, n = n0 + 16 * (t % NJ) + 4 * lg;
+    if (m < m1 && n < a.N) {
+      if (a.xs) o.sx = a.xs[m];
+      o.ws = column4(a.ws + (size_t)e * a.N, n, a.N, a.vec);
+      o.bias = column4(a.bias ? a.bias + (size_t)e * a.N : nullptr, n, a.N, a.vec);
+      if (a.vec && a.res) o.res = residual_raw(a, m, n);
+    }
+    return o;
+  };
+  constexpr bool AHEAD = MI * NJ <= WK;
+  Ends ahead;
   const int sf = s1 < full ? s1 : full;
   int s = s0;
   if (s + U <= sf) load(0, s);
+  if (AHEAD && wave < MI * NJ) ahead = ends(wave);
   for (; s + 3 * U <= sf; s += 2 * U) {
     load(1, s + U);
     multiply(0);
@@ -294,15 +323,22 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
     multiply(0);
     s += U;
   }
-  for (; s < s1; ++s) {
-    const int k = s * KB, avail = a.K - k - 16 * lg;  // the end of K: zeros past it
-    v4i vx[MI], vw[NJ];
+  // what is left: fewer than U whole steps, and the end of K with zeros past it
 #pragma unroll
-    for (int i = 0; i < MI; ++i) vx[i] = load_tail16<ODD>(xp[i] + k, avail, k + 16 * lg);
+  for (int u = 0; u + 1 < U; ++u)
+    if (s + u < sf) load_step(0, u, s + u);
+  v4i ex[MI], ew[NJ];
+  if (s1 > full) {
+    const int k = full * KB + 16 * lg, avail = a.K - k;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) vw[j] = load_tail16<ODD>(wp[j] + k, avail, k + 16 * lg);
-    product(vx, vw);
+    for (int i = 0; i < MI; ++i) ex[i] = load_tail16<ODD>(xp[i] + full * KB, avail, k);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) ew[j] = load_tail16<ODD>(wp[j] + full * KB, avail, k);
   }
+#pragma unroll
+  for (int u = 0; u + 1 < U; ++u)
+    if (s + u < sf) multiply_step(0, u);
+  if (s1 > full) product(ex, ew);
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -313,19 +349,17 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
 #pragma unroll
     for (int k = 1; k < WK; ++k) s += part[k][t][lane];
     const int m = m0 + 16 * (t / NJ) + lr, n = n0 + 16 * (t % NJ) + 4 * lg;
+    if (!AHEAD) ahead = ends(t);
     if (m < m1 && n < a.N) {
-      const float sx = a.xs ? a.xs[m] : 1.f;
-      const v4f ws = column4(a.ws + (size_t)e * a.N, n, a.N, a.vec);
-      const v4f b = column4(a.bias ? a.bias + (size_t)e * a.N : nullptr, n, a.N, a.vec);
-      v4f v, r = {0.f, 0.f, 0.f, 0.f};
-      if (a.vec && a.res) r = residual4(a, m, n);
+      v4f v;
       with_act(a.act, [&](auto act) {
-        v = scaled4<decltype(act)::value>(v4f{(float)s[0], (float)s[1], (float)s[2], (float)s[3]}, sx, ws, b);
+        v = scaled4<decltype(act)::value>(v4f{(float)s[0], (float)s[1], (float)s[2], (float)s[3]}, ahead.sx, ahead.ws,
+                                          ahead.bias);
       });
       if (!a.vec)
         put4_any(a, m, n, v);
       else
-        put4(a, m, n, a.res ? v + r : v);
+        put4(a, m, n, a.res ? v + residual_value(a, ahead.res) : v);
     }
   }
 }
