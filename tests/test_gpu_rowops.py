@@ -213,12 +213,14 @@ def test_linear_offsets_past_32_bits(gpu, t):
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("M,N,ldr", [(300, 1700, 1 << 21), (300, 1700, (1 << 21) + 4), (700, 1028, 1028), (700, 1028, 1029)])
-def test_linear_residual_rows_far_apart(gpu, out, M, N, ldr):
+@pytest.mark.parametrize("M,N,K,ldr", [(300, 1700, 192, 1 << 21), (300, 1700, 192, (1 << 21) + 4),
+                                       (700, 1028, 192, 1028), (700, 1028, 193, 1032), (700, 1028, 193, 1029),
+                                       (2500, 4000, 2048, 4000), (2500, 4000, 2049, 4004)])
+def test_linear_residual_strides(gpu, out, M, N, K, ldr):
     """A residual whose rows lie further apart than a tile's 32-bit offsets
-    reach, up to there, and off 4 elements."""
+    reach, up to there, and off 4 elements; rows of codes on and off 16 bytes."""
     rng = np.random.default_rng([M, ldr])
-    c = case(rng, "s8", M, N, 192, out)
+    c = case(rng, "s8", M, N, K, out)
     big = torch.empty((M - 1) * ldr + N, dtype=out, device="cuda")
     res = big.as_strided((M, N), (ldr, 1))
     res.copy_(c["res"])
@@ -633,6 +635,36 @@ def test_rowops_repeat_and_other_stream(gpu):
     torch.cuda.current_stream().wait_stream(side)
     for u, v, w in zip(a, b, c):
         assert torch.equal(u, v) and torch.equal(u, w)
+
+
+def test_rowops_on_two_streams_at_once(gpu):
+    """Calls that run beside each other do not share anything."""
+    from dlq_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w = torch.randint(-60, 60, (9000, 512), generator=g, device="cuda", dtype=torch.int8)
+    ws = torch.rand(9000, generator=g, device="cuda") * 0.01
+    xs = [torch.randn(200, 512, generator=g, device="cuda") for _ in range(2)]
+
+    def run(x):
+        q, s = ops.quantize_rows_dyn_s8(x)
+        y = ops.linear_act_s8(q, w, s, ws, None, "silu")
+        r = ops.logprobs(y, None, 9)
+        return [q, s, y, r.entropy, r.top_idx, r.top_logprob]
+
+    want = [run(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(xs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            for u, v in zip(r, want[i]):
+                assert torch.equal(u, v)
 
 
 @pytest.mark.parametrize("t", ["s8", "f8"])
