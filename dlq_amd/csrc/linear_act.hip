@@ -427,8 +427,20 @@ __device__ __forceinline__ const int8_t* uniform(const int8_t* p) {
   return (const int8_t*)((unsigned long long)hi << 32 | lo);
 }
 
-template <bool F8, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE, bool RES>
-__global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const LinearArgs a, int nbm, int nbn) {
+template <int WN, int WM, int NI, int MJ, int KB, int SLOTS, bool RES>
+struct TileLds {
+  static constexpr int NW = WN * WM, SLOT = 32 * (WN * NI + WM * MJ) * KB;
+  static constexpr int PITCH = NI * 32 * 4 + 16;  // epilogue staging: 32 rows of a wave's columns
+  // lanes per row, rows per instruction, instructions per 32 rows, in flight of the epilogue
+  static constexpr int LPR = NI * 8, RPI = 64 / LPR, NP = 32 / RPI, U = 4;
+  static_assert(NP % U == 0, "rows of a staging pass");
+  static constexpr int EPILOGUE = NW * (32 * PITCH + (RES ? NP * 1024 : 0));  // staging, residual
+  static constexpr int BYTES = SLOTS * SLOT > EPILOGUE ? SLOTS * SLOT : EPILOGUE;
+};
+
+// Columns from n0 on of rows [m0, m1) of expert e.
+template <bool F8, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, bool RES>
+__device__ __forceinline__ void linear_tile(const LinearArgs& a, int e, int m0, int m1, int n0, int8_t* lds) {
   typedef TileMma<F8, NV> MM;
   typedef typename MM::acc_t acc_t;
   typedef typename MM::sum4 sum4;
@@ -441,28 +453,11 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
   static_assert(KB == 128 || KB == 64, "chunk swizzle");
   static_assert(NW % 2 == 0 && TN % (RPP * NW) == 0 && TM % (RPP * NW) == 0, "pieces per wave");
   static_assert(PP * (SLOTS - 1) <= 63, "counted waits");
-  constexpr int PITCH = NI * 32 * 4 + 16;  // epilogue staging: 32 rows of a wave's columns
-  // lanes per row, rows per instruction, instructions per 32 rows, in flight of the epilogue
-  constexpr int LPR = NI * 8, RPI = 64 / LPR, NP = 32 / RPI, U = 4;
-  static_assert(NP % U == 0, "rows of a staging pass");
-  constexpr int EPILOGUE = NW * (32 * PITCH + (RES ? NP * 1024 : 0));  // staging, residual
-  __shared__ __attribute__((aligned(16))) int8_t lds[SLOTS * SLOT > EPILOGUE ? SLOTS * SLOT : EPILOGUE];
+  typedef TileLds<WN, WM, NI, MJ, KB, SLOTS, RES> L;
+  constexpr int PITCH = L::PITCH, LPR = L::LPR, RPI = L::RPI, NP = L::NP, U = L::U;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, lh = lane >> 5, wn = wave % WN, wm = wave / WN;
-  // each XCD takes a run of tiles, down groups of 4 row blocks column by column
-  constexpr int GROW = 4;
-  const int l = xcd_remap(blockIdx.x, gridDim.x);
-  const int grp = l / (GROW * nbn), r0 = grp * GROW;
-  const int gsz = nbm - r0 < GROW ? nbm - r0 : GROW, li = l - grp * GROW * nbn;
-  const int mt = r0 + li % gsz, n0 = li / gsz * TN;
-  int e = 0, m0 = mt * TM, m1 = a.M;
-  if (a.E) {
-    if (!expert_tile<TM>(a, mt, e, m0, m1)) return;
-    e = __builtin_amdgcn_readfirstlane(e);
-    m0 = __builtin_amdgcn_readfirstlane(m0);
-    m1 = __builtin_amdgcn_readfirstlane(m1);
-  }
   const int8_t* wbase = uniform(a.w + ((size_t)e * a.N + n0) * a.ldw);
   const int8_t* xbase = uniform(a.x + (size_t)m0 * a.ldx);
 
@@ -774,6 +769,60 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
   }
 }
 
+// The l-th tile of TN x TM in an order that shares operands: down groups of 4
+// row blocks, column by column.  false: it has no rows.
+template <int TN, int TM>
+__device__ __forceinline__ bool tile_at(const LinearArgs& a, int l, int nbm, int nbn, int& e, int& m0, int& m1,
+                                        int& n0) {
+  constexpr int GROW = 4;
+  const int grp = l / (GROW * nbn), r0 = grp * GROW;
+  const int gsz = nbm - r0 < GROW ? nbm - r0 : GROW, li = l - grp * GROW * nbn;
+  const int mt = r0 + li % gsz;
+  n0 = li / gsz * TN;
+  e = 0;
+  m0 = mt * TM;
+  m1 = a.M;
+  if (a.E) {
+    if (!expert_tile<TM>(a, mt, e, m0, m1)) return false;
+    e = __builtin_amdgcn_readfirstlane(e);
+    m0 = __builtin_amdgcn_readfirstlane(m0);
+    m1 = __builtin_amdgcn_readfirstlane(m1);
+  }
+  return true;
+}
+
+template <bool F8, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE, bool RES>
+__global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const LinearArgs a, int nbm, int nbn) {
+  __shared__ __attribute__((aligned(16))) int8_t lds[TileLds<WN, WM, NI, MJ, KB, SLOTS, RES>::BYTES];
+  int e, m0, m1, n0;  // each XCD takes a run of tiles
+  if (!tile_at<32 * WN * NI, 32 * WM * MJ>(a, xcd_remap(blockIdx.x, gridDim.x), nbm, nbn, e, m0, m1, n0)) return;
+  linear_tile<F8, REG, WN, WM, NI, MJ, NV, KB, SLOTS, RES>(a, e, m0, m1, n0, lds);
+}
+
+// 256 x 256 tiles, from the `whole`-th on in four workgroups of 128 x 128, which
+// start as CUs come free: a last round that would leave most of them idle takes
+// a third of the time.  16384 rows over 8 experts of 4096 x 4096 e4m3 318 -> 288
+// us, 4096 x 5120 x 16384 int8 335 -> 292, 4096 x 4608 x 4096 96 -> 87 (as a
+// launch behind the first one it gained nothing: that waits for the slowest).
+template <bool F8, bool RES>
+__global__ __launch_bounds__(256, 1) void linear_tile_quarters_kernel(const LinearArgs a, int nbm, int nbn, int whole) {
+  constexpr int B0 = TileLds<2, 2, 4, 4, 128, 2, RES>::BYTES, B1 = TileLds<2, 2, 2, 2, 128, 4, RES>::BYTES;
+  __shared__ __attribute__((aligned(16))) int8_t lds[B0 > B1 ? B0 : B1];
+  int e, m0, m1, n0;
+  const int b = blockIdx.x;
+  if (b < whole) {
+    if (!tile_at<256, 256>(a, xcd_remap(b, whole), nbm, nbn, e, m0, m1, n0)) return;
+    linear_tile<F8, false, 2, 2, 4, 4, 2, 128, 2, RES>(a, e, m0, m1, n0, lds);
+  } else {
+    const int q = b - whole;
+    if (!tile_at<256, 256>(a, whole + q / 4, nbm, nbn, e, m0, m1, n0)) return;
+    m0 += q % 2 * 128;
+    n0 += q / 2 % 2 * 128;
+    if (m0 >= m1 || n0 >= a.N) return;
+    linear_tile<F8, false, 2, 2, 2, 2, 4, 128, 4, RES>(a, e, m0, m1, n0, lds);
+  }
+}
+
 // row tiles of BM that the rows can need; grouped: each expert adds at most
 // one part-filled tile, and no tile is empty
 long row_tiles(const LinearArgs& a, int BM) {
@@ -834,6 +883,7 @@ int num_cus() {
 //   2276 x 953 x 16128  471   258   177    83     77    112    194
 //   2048 x 4096 x 4096  450   232   125    70     54     42     62
 //   4096 x 4096 x 4096  897   455   241   127    106     83     69
+//   (256: the last round whole)
 //   K odd:                                 64   128 x 64
 //   32 x 4096 x 4099     16    19    32    26
 //   64 x 4096 x 4099     27    18    39    29     39
@@ -862,8 +912,16 @@ float tiles_of_rows(const LinearArgs& a, int tm) {
   return t < a.M ? t : (float)a.M;
 }
 
+// Tiles of 256 x 256 whose last round, `rest` of them, runs in quarters of
+// 128 x 128, one on a CU: what that takes.
+float quarters_cost(const TileCost& t128, float rest, float cus, float k) {
+  return __builtin_ceilf(4.f * rest / cus) * (t128.one * k + t128.fixed);
+}
+
+// whole: how many tiles of the best kind's stay whole if the others run in
+// quarters (-1: all)
 template <int N>
-int best_tile(const LinearArgs& a, const TileCost (&tiles)[N]) {
+int best_tile(const LinearArgs& a, const TileCost (&tiles)[N], int& whole) {
   int best = 0;
   float least = 0.f;
   const float cus = (float)num_cus(), k = a.K / 1024.f;
@@ -871,26 +929,51 @@ int best_tile(const LinearArgs& a, const TileCost (&tiles)[N]) {
     const TileCost& t = tiles[i];
     const float wgs = tiles_of_rows(a, t.tm) * (float)((a.N + t.tn - 1) / t.tn), round = cus * t.per_cu;
     const float rounds = __builtin_floorf(wgs / round), rest = wgs - rounds * round;
-    const float c = rounds * (t.two * k + t.fixed) + (rest <= 0.f ? 0.f : (rest <= cus ? t.one : t.two) * k + t.fixed);
+    float last = rest <= 0.f ? 0.f : (rest <= cus ? t.one : t.two) * k + t.fixed;
+    bool quarters = false;
+    if (t.tn == 256 && rounds > 0.f && rest > 0.f) {
+      const float q = quarters_cost(tiles[1], rest, cus, k);
+      quarters = q < last;
+      if (quarters) last = q;
+    }
+    const float c = rounds * (t.two * k + t.fixed) + last;
     if (i == 0 || c < least) {
       least = c;
       best = i;
+      whole = quarters ? (int)(rounds * round) : -1;
     }
   }
   return best;
 }
 
 template <bool F8>
+hipError_t launch_quarters(const LinearArgs& a, int whole, hipStream_t s) {
+  const long nbn = (a.N + 255) / 256, nbm = row_tiles(a, 256);
+  if (whole > nbm * nbn) whole = (int)(nbm * nbn);
+  const long grid = whole + 4 * (nbm * nbn - whole);
+  if (!grid_fits(grid, 256)) return hipErrorInvalidValue;
+  if (a.vec && a.res)
+    hipLaunchKernelGGL((linear_tile_quarters_kernel<F8, true>), dim3((unsigned)grid), dim3(256), 0, s, a, (int)nbm,
+                       (int)nbn, whole);
+  else
+    hipLaunchKernelGGL((linear_tile_quarters_kernel<F8, false>), dim3((unsigned)grid), dim3(256), 0, s, a, (int)nbm,
+                       (int)nbn, whole);
+  return hipGetLastError();
+}
+
+template <bool F8>
 hipError_t launch_best_tile(const LinearArgs& a, bool dma, hipStream_t s) {
+  int whole;
   if (!dma) {
-    if (best_tile(a, kRegTiles) == 0) return launch_tile<F8, true, 2, 2, 1, 1, 4, 128, 2, 2>(a, s);
+    if (best_tile(a, kRegTiles, whole) == 0) return launch_tile<F8, true, 2, 2, 1, 1, 4, 128, 2, 2>(a, s);
     return launch_tile<F8, true, 2, 2, 2, 1, 2, 128, 2, 2>(a, s);
   }
-  switch (best_tile(a, kDmaTiles<F8>)) {
+  switch (best_tile(a, kDmaTiles<F8>, whole)) {
     case 0: return launch_tile<F8, false, 2, 2, 1, 1, F8 ? 2 : 4, 128, 5, 2>(a, s);
     case 1: return launch_tile<F8, false, 2, 2, 2, 2, 4, 128, 4, 1>(a, s);
     case 2: return launch_tile<F8, false, 2, 2, 2, 2, 2, 128, 2, 2>(a, s);
-    default: return launch_tile<F8, false, 2, 2, 4, 4, 2, 128, 2, 1>(a, s);
+    default:
+      return whole > 0 ? launch_quarters<F8>(a, whole, s) : launch_tile<F8, false, 2, 2, 4, 4, 2, 128, 2, 1>(a, s);
   }
 }
 

@@ -230,6 +230,18 @@ def test_linear_residual_strides(gpu, out, M, N, K, ldr):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("res", [0, 1])
+def test_linear_last_round_of_tiles(gpu, t, res):
+    """More tiles than CUs, the rest in smaller ones, ragged on both sides."""
+    rng = np.random.default_rng(res)
+    M, N, K = 4100, 4500, 1040
+    c = case(rng, t, M, N, K, torch.bfloat16, res=bool(res))
+    y = linear(t)[0](dev(c["x"]), dev(c["w"]), dev(c["xs"]), dev(c["ws"]), dev(c["bias"]), "silu", dev(c["res"]),
+                     out_dtype=torch.bfloat16)
+    close(y, *product64(**c, act="silu", out_dtype=torch.bfloat16))
+
+
 def grouped_reference(c, off, t, act, out, T):
     y = torch.full((T, c["w"].shape[1]), 3.0, dtype=torch.float64)
     tol = torch.zeros_like(y)
@@ -283,6 +295,19 @@ def test_grouped_many(gpu, t, E, T):
     linear(t)[1](dev(c["x"]), torch.tensor(off, dtype=torch.int32, device="cuda"), dev(c["w"]), dev(c["xs"]),
                  dev(c["ws"]), dev(c["bias"]), "gelu_tanh", out=y)
     close(y, *grouped_reference(c, off, t, "gelu_tanh", torch.float32, T))
+
+
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("off", [[0, 1500, 1501, 4300], [7, 7, 4400, 4400], [0, 130, 300, 520]])
+def test_grouped_last_round_of_tiles(gpu, t, off):
+    """The same by expert: most rows, one expert's, and far fewer than the launch allows for."""
+    rng = np.random.default_rng(off[1])
+    T, N, K = 4400, 4612, 1040
+    c = grouped_case(rng, t, 3, T, N, K, torch.bfloat16)
+    y = torch.full((T, N), 3.0, dtype=torch.bfloat16, device="cuda")
+    linear(t)[1](dev(c["x"]), torch.tensor(off, dtype=torch.int32, device="cuda"), dev(c["w"]), dev(c["xs"]),
+                 dev(c["ws"]), dev(c["bias"]), "none", dev(c["res"]), out=y)
+    close(y, *grouped_reference(c, off, t, "none", torch.bfloat16, T))
 
 
 def test_grouped_offsets_outside(gpu):
