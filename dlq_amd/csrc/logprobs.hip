@@ -464,7 +464,8 @@ __device__ __forceinline__ unsigned wave_nth(const unsigned (&key)[4], int n) {
 // or above it -- `top` or a few more -- are read again.  Where more logits reach
 // it than the list holds, the list is cut to its `top` largest whenever it
 // fills up; where many groups are at the bound (masked rows, equal logits), what
-// equals it is taken in order from its first chunk on.
+// equals it is taken in order, from the chunks that have a group at or above it
+// (one below a larger logit of its group shows in no head).
 template <bool BF16>
 __global__ __launch_bounds__(256, 8) void logprobs_join_kernel(const LogprobArgs a) {
   constexpr int EPV = kEpv<BF16>, QUAD = 4 * kLane, SZ = BF16 ? 2 : 4;
@@ -541,7 +542,7 @@ __global__ __launch_bounds__(256, 8) void logprobs_join_kernel(const LogprobArgs
         const int h = h0 + 256 * r + tid;
         const unsigned k = h < total ? value_key(h0 ? heads[h] : early[r]) : 0u;
         if (k >= (unsigned)(above >> 32)) groups[atomicAdd(&found, 1)] = h;
-        if (tied && k == v) atomicMin(&start, h / 64);  // their first chunk
+        if (tied && k >= v) atomicMin(&start, h / 64);  // the first chunk that may hold one
       }
       __syncthreads();
       again = !tied && found > kTied && above == (u64)v << 32;
@@ -604,9 +605,14 @@ __global__ __launch_bounds__(256, 8) void logprobs_join_kernel(const LogprobArgs
   }
   int have = count;
   __syncthreads();
-  int step = 128;  // most often enough, and a short list
+  // the first step is most often enough, and leaves a short list
   long long j0 = v == none ? 0 : (long long)start * kGroupChunk;
-  for (; tied && have < top && j0 < a.K; j0 += step, step = 512) {
+  for (int step = 128; tied && have < top && j0 < a.K; j0 += step, step = 512 - (int)(j0 % 512)) {
+    if (j0 % kGroupChunk == 0 &&
+        !__syncthreads_or(value_key(heads[j0 / kGroupChunk * 64 + (tid & 63)]) >= v)) {
+      step = kGroupChunk;
+      continue;
+    }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const long long j = j0 + 256 * r + tid;

@@ -535,6 +535,25 @@ def test_logprobs_ties_at_the_borders(gpu, xt, K, top):
     assert np.array_equal(ops.logprobs(x[8:].cuda(), None, top).top_idx.cpu().numpy(), alternatives(x[8:], top))
 
 
+@pytest.mark.parametrize("xt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("K,spikes,ones,top", [
+    (32768, [0], [1, *range(8192, 32768)], 5),                  # the first 1 lies beside the row's largest
+    (32768, [0, 9000], [3, 9001, *range(16384, 32768)], 4),     # so do the first two, a chunk each
+    (65537, [70], [71, *range(65536 - 20000, 65537)], 64),      # chunks without one lie between
+    (262144, [5], [6, *range(8192, 262144, 100)], 7),           # more heads than one step takes
+    (262144, [8195 * 17], [8195 * 17 + 1, *range(8192 * 18, 262144)], 3),  # of a later step
+    (300007, [0, 140000], [140001, *range(290000, 300007, 2)], 20)])
+def test_logprobs_ties_beside_a_larger_logit(gpu, xt, K, spikes, ones, top):
+    """Equal logits of which the first stand in a group of 128 that holds a
+    larger one as well, so that its largest does not tell of them."""
+    x = torch.full((2, K), -5.0)
+    x[1] = -math.inf
+    x[:, ones] = 1.0
+    x[:, spikes] = 2.0
+    tokens = torch.tensor([ones[0], ones[-1]], dtype=torch.int32)
+    check_logprobs(x.to(xt), tokens, top)
+
+
 @pytest.mark.parametrize("K", [40, 5000, 30000])
 def test_logprobs_not_finite(gpu, K):
     """NaN and +inf make their row's numbers NaN, the order stays defined."""
