@@ -447,11 +447,12 @@ def block_l1_f8(x: torch.Tensor, w1: torch.Tensor, alpha1: torch.Tensor, beta1: 
 
 # ------------------------------------------- row operators (tokens as rows)
 # include/dlq.h "Row operators of quantised transformer serving".  Tensors may
-# be row-strided views (unit stride within a row); all of a call's tensors lie
-# on one device, which need not be the current one; the work goes to that
-# device's current stream.
+# be row-strided views (unit stride within a row; sizes and strides up to
+# 2^31 - 1, refused beyond); all of a call's tensors lie on one device, which
+# need not be the current one; the work goes to that device's current stream.
 
 _TYPES = {torch.float32: DLQ_T_F32, torch.bfloat16: DLQ_T_BF16}
+_INT_MAX = 2**31 - 1  # ctypes cuts a larger number to its low 32 bits without a word
 
 
 def _placed(t, name: str, dtypes, dev) -> None:
@@ -474,6 +475,8 @@ def _rows(t: torch.Tensor, name: str, dtypes, dev, rows=None, cols=None):
         ld = c
     if (c > 1 and unit != 1) or ld < c:
         raise ValueError(f"{name}: rows must have unit stride and not overlap, strides {t.stride()}")
+    if ld > _INT_MAX or r > _INT_MAX:
+        raise ValueError(f"{name}: {r} rows at stride {ld}, the library's sizes and strides end at {_INT_MAX}")
     return r, c, ld
 
 
@@ -515,6 +518,8 @@ def _quantize_rows_dyn(what, fn, dtype, x, ld):
     rows, cols, ldx = _rows(x, "x", _TYPES, dev)
     if ld is None:
         ld = cols
+    elif not cols <= ld <= _INT_MAX:
+        raise ValueError(f"ld: {ld}, expected {cols} to {_INT_MAX}")
     q = x.new_empty((rows, ld), dtype=dtype)
     scale = x.new_empty(rows, dtype=torch.float32)
     _launch(what, fn, dev, x.data_ptr(), _TYPES[x.dtype], rows, cols, ldx, q.data_ptr(), ld, scale.data_ptr())
@@ -550,6 +555,8 @@ def _linear(what, fn, code, x, w, x_scale, w_scale, bias, act, residual, out_dty
         if not isinstance(w, torch.Tensor) or w.dim() != 3 or w.shape[2] != K:
             raise ValueError(f"w: expected a tensor [E, N, {K}]")
         E, N, ldw = w.shape
+        if max(E, N) > _INT_MAX:
+            raise ValueError(f"w: shape {tuple(w.shape)}, the library's sizes end at {_INT_MAX}")
         _vector(w, "w", (code,), dev, w.shape)
         per_column = (E, N)
     if w_scale is None:
@@ -632,6 +639,8 @@ def logprobs(x: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0) 
     (<= 64) largest with their indices, equal ones by ascending index."""
     dev = _device(x, "x")
     rows, K, ldx = _rows(x, "x", _TYPES, dev)
+    if not 0 <= top <= 64:
+        raise ValueError(f"top: {top}, expected 0 to 64")
     t = _vector(tokens, "tokens", _I32, dev, (rows,))
     lp = None if t is None else x.new_empty(rows, dtype=torch.float32)
     ent = x.new_empty(rows, dtype=torch.float32)

@@ -758,6 +758,20 @@ def test_rowops_graph(gpu, t):
                 assert torch.equal(a, b), (rep, k)
 
 
+def test_ops_refuse_far_strides(gpu):
+    """Two rows 2^32 + K elements apart: refused, not taken for rows K apart."""
+    from dlq_amd import ops
+    K = 64
+    big = torch.zeros(2 ** 32 + 2 * K, dtype=torch.int8, device="cuda")
+    x = big.as_strided((2, K), (2 ** 32 + K, 1))
+    w, s = torch.zeros(8, K, dtype=torch.int8, device="cuda"), torch.ones(8, device="cuda")
+    with pytest.raises(ValueError, match="strides end at"):
+        ops.linear_act_s8(x, w, None, s)
+    assert ops.linear_act_s8(x[1:], w, None, s).shape == (1, 8)  # one row has no stride
+    del big, x
+    torch.cuda.empty_cache()
+
+
 def test_ops_check_devices_and_shapes(gpu):
     from dlq_amd import ops
     x = torch.zeros(4, 32, dtype=torch.int8, device="cuda")

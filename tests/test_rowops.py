@@ -115,3 +115,72 @@ def test_ops_refuse_host_tensors():
         ops.quantize_rows_dyn_s8(torch.zeros(2, 8))
     with pytest.raises(TypeError):
         ops.logprobs(torch.zeros(2, 8))
+
+
+class Placed(torch.Tensor):
+    """Passes for a tensor on device 0; without memory."""
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+
+def placed(dtype, rows, cols, ld=None):
+    ld = cols if ld is None else ld
+    big = torch.empty(max(rows - 1, 0) * ld + cols, dtype=dtype, device="meta")
+    return big.as_strided((rows, cols), (ld, 1)).as_subclass(Placed)
+
+
+@pytest.mark.parametrize("ld", [2 ** 31, 2 ** 32 + 32, 2 ** 32 + 2 ** 31])
+def test_ops_refuse_strides_past_32_bits(ld):
+    """A row stride that an int does not hold is refused, not cut to its low bits."""
+    from dlq_amd import ops
+    x, w, s = placed(torch.int8, 4, 32), placed(torch.int8, 8, 32), placed(torch.float32, 1, 8)[0]
+    far = lambda t, c: placed(t, 4, c, ld)  # noqa: E731
+    e = placed(torch.int32, 1, 2)[0]
+    word = "strides end at 2147483647"
+    for f in (ops.linear_act_s8, ops.linear_act_f8):
+        code = torch.int8 if f is ops.linear_act_s8 else torch.uint8
+        y, v = placed(code, 4, 32), placed(code, 8, 32)
+        with pytest.raises(ValueError, match="x: .*" + word):
+            f(far(code, 32), v, None, s)
+        with pytest.raises(ValueError, match="w: .*" + word):
+            f(y, far(code, 32), None, s[:4])
+        with pytest.raises(ValueError, match="out: .*" + word):
+            f(y, v, None, s, out=far(torch.float32, 8))
+        with pytest.raises(ValueError, match="residual: .*" + word):
+            f(y, v, None, s, residual=far(torch.float32, 8))
+    with pytest.raises(ValueError, match="x: .*" + word):
+        ops.linear_grouped_s8(far(torch.int8, 32), e, w[None], None, s[None])
+    with pytest.raises(ValueError, match="out: .*" + word):
+        ops.linear_grouped_s8(x, e, w[None], None, s[None], out=far(torch.float32, 8))
+    for f in (ops.quantize_rows_dyn_s8, ops.quantize_rows_dyn_f8):
+        with pytest.raises(ValueError, match="x: .*" + word):
+            f(far(torch.bfloat16, 32))
+        with pytest.raises(ValueError, match="ld: "):
+            f(placed(torch.bfloat16, 4, 32), ld=ld)
+    with pytest.raises(ValueError, match="x: .*" + word):
+        ops.logprobs(far(torch.float32, 32))
+
+
+def test_ops_refuse_sizes_past_32_bits():
+    from dlq_amd import ops
+    n = 2 ** 32 + 1
+    s = placed(torch.float32, 1, 8)[0]
+    for x in (placed(torch.int8, n, 1), placed(torch.int8, 1, n)):
+        with pytest.raises(ValueError, match="sizes"):
+            ops.linear_act_s8(x, placed(torch.int8, 8, x.shape[1]), None, s)
+    with pytest.raises(ValueError, match="sizes"):
+        ops.linear_act_s8(placed(torch.int8, 4, 1), placed(torch.int8, n, 1), None, placed(torch.float32, 1, n)[0])
+    with pytest.raises(ValueError, match="sizes"):
+        ops.linear_grouped_s8(placed(torch.int8, 4, 1), placed(torch.int32, 1, 2)[0], placed(torch.int8, n, 1)[None],
+                              None, placed(torch.float32, 1, n))
+    with pytest.raises(ValueError, match="sizes"):
+        ops.quantize_rows_dyn_s8(placed(torch.float32, n, 1))
+    with pytest.raises(ValueError, match="ld: "):
+        ops.quantize_rows_dyn_s8(placed(torch.float32, 4, 32), ld=31)
+    with pytest.raises(ValueError, match="sizes"):
+        ops.logprobs(placed(torch.float32, n, 1))
+    for top in (-1, 65, 2 ** 32 + 3):
+        with pytest.raises(ValueError, match="top"):
+            ops.logprobs(placed(torch.float32, 4, 100), None, top)
