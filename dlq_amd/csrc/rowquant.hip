@@ -38,9 +38,10 @@ struct Vec {
     r = *(const v4i_any*)((const char*)x + i * (BF16 ? 2 : 4));
   }
   // the last values of a row, from column c on; zeros behind them
-  __device__ __forceinline__ void load_end(const void* x, size_t x0, int c, int cols) {
+  __device__ __forceinline__ void load_end(const void* x, size_t x0, unsigned c, unsigned cols) {
     constexpr int S = BF16 ? 2 : 4;
-    r = load_tail16<false>((const char*)x + (x0 + c) * S, (cols - c) * S < 16 ? (cols - c) * S : 16, c * S);
+    const int left = (int)(cols - c) * S;
+    r = load_tail16<false>((const char*)x + (x0 + c) * S, left < 16 ? left : 16, c < 16 ? (int)c * S : 16);
   }
   __device__ __forceinline__ unsigned most() const {
     unsigned u = 0;
@@ -69,14 +70,15 @@ struct Vec {
 // NW waves per row (a workgroup; 1: four rows per workgroup, no barriers),
 // KEEP columns of it in registers.
 template <bool BF16, bool F8, int NW, int KEEP>
-__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_kernel(const void* __restrict__ x, int rows, int cols, int ldx,
-                                                                uint8_t* __restrict__ q, int ldq,
-                                                                float* __restrict__ scale) {
+__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_kernel(
+    const void* __restrict__ x, int rows, unsigned cols, int ldx, uint8_t* __restrict__ q, unsigned ldq,
+    float* __restrict__ scale) {
+  // columns are unsigned: cols and ldq end at 2^31 - 1, and a step beyond them must not wrap
   typedef Vec<BF16> V;
   constexpr int TPR = 64 * NW, N = V::N, SPAN = TPR * N;  // columns of one load of all lanes
   constexpr int NV = KEEP / SPAN;                         // loads kept in registers
   __shared__ unsigned wmax[NW];
-  const int t = threadIdx.x % TPR;
+  const unsigned t = threadIdx.x % TPR;
   const int row = NW == 1 ? (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6) : (int)blockIdx.x;
   if (NW == 1 && row >= rows) return;
   const size_t x0 = (size_t)row * ldx;
@@ -84,7 +86,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_ker
   V v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = i * SPAN + t * N;
+    const unsigned c = i * SPAN + t * N;
     if (c + N <= cols)
       v[i].load(x, x0 + c);
     else if (c < cols)
@@ -94,7 +96,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_ker
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (i * SPAN + t * N < cols) u = max(u, v[i].most());
-  for (int c = NV * SPAN + t * N; c < cols; c += SPAN) {
+  for (unsigned c = NV * SPAN + t * N; c < cols; c += SPAN) {
     V w;
     if (c + N <= cols)
       w.load(x, x0 + c);
@@ -114,7 +116,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_ker
   const float s = bad ? __uint_as_float(0x7fc00000u) : none ? 1.f : __fdiv_rn(a, F8 ? 448.f : 127.f);
   const float inv = none ? 0.f : __fdiv_rn(1.f, s);
   if (t == 0) scale[row] = s;
-  const auto put = [&](const V& w, int c) {
+  const auto put = [&](const V& w, unsigned c) {
     v2u o = w.template codes<F8>(inv);
     if (bad) o = v2u{0u, 0u};  // 0 * inf
     if (c + N <= cols) {
@@ -130,10 +132,10 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_ker
   };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = i * SPAN + t * N;
+    const unsigned c = i * SPAN + t * N;
     if (c < cols) put(v[i], c);
   }
-  for (int c = NV * SPAN + t * N; c < cols; c += SPAN) {
+  for (unsigned c = NV * SPAN + t * N; c < cols; c += SPAN) {
     V w;
     if (c + N <= cols)
       w.load(x, x0 + c);
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_ker
       w.load_end(x, x0, c, cols);
     put(w, c);
   }
-  for (int c = cols + t; c < ldq; c += TPR) qr[c] = 0;
+  for (unsigned c = cols + t; c < ldq; c += TPR) qr[c] = 0;
 }
 
 template <bool BF16, bool F8>

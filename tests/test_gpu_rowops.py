@@ -409,6 +409,34 @@ def test_quantize_rows_dyn_edges(gpu, t, cols):
     assert np.array_equal(got.numpy(), rq)
 
 
+@pytest.mark.parametrize("t,cols,ld", [("s8", 2 ** 31 - 1, 2 ** 31 - 1), ("f8", 2 ** 31 - 8000, 2 ** 31 - 1),
+                                       ("s8", 100, 2 ** 31 - 1), ("f8", 20000, 2 ** 31 - 500)])
+def test_quantize_rows_dyn_longest_rows(gpu, t, cols, ld):
+    """One row up to the last column an int numbers, bf16; codes and padding end where the row does."""
+    from dlq_amd import ops
+    x = torch.empty(1, cols, dtype=torch.bfloat16, device="cuda")
+    piece = 1 << 28
+    for c in range(0, cols, piece):
+        x[0, c:c + piece] = (torch.arange(min(piece, cols - c), device="cuda", dtype=torch.int32) % 509 - 254).bfloat16()
+    x[0, -1] = 300.0
+    q, s = (ops.quantize_rows_dyn_s8 if t == "s8" else ops.quantize_rows_dyn_f8)(x, ld=ld)
+    m = 127.0 if t == "s8" else 448.0
+    scale = torch.tensor(300.0, device="cuda") / torch.tensor(m, device="cuda")
+    assert q.shape == (1, ld) and s.item() == scale.item()
+    inv = torch.ones_like(scale) / scale
+    for c in range(0, cols, piece):
+        v = (x[0, c:c + piece].float() * inv).clamp(-m, m)
+        want = v.round().to(torch.int8) if t == "s8" else v.to(F8).view(torch.uint8)
+        got = q[0, c:min(c + piece, cols)]
+        if t == "f8":  # zeros of either sign
+            got, want = got & (0x7F + 0x80 * (got != 0x80)), want & (0x7F + 0x80 * (want != 0x80))
+        assert torch.equal(got, want), c
+        del v, want, got
+    assert not q[0, cols:].any()
+    del x, q
+    torch.cuda.empty_cache()
+
+
 # -------------------------------------------------------- log probabilities
 
 def lp_bounds(x):
