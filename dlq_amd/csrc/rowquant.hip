@@ -146,20 +146,28 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void quantize_rows_dyn_ker
   for (unsigned c = cols + t; c < ldq; c += TPR) qr[c] = 0;
 }
 
+template <bool BF16, bool F8, int NW, int KEEP>
+hipError_t launch_as(const void* x, int rows, int cols, int ldx, uint8_t* q, int ldq, float* scale, hipStream_t s) {
+  constexpr int ROWS = NW == 1 ? 4 : 1, THREADS = NW == 1 ? 256 : NW * 64;
+  constexpr long long MOST = (1LL << 21) * ROWS;  // rows of one launch, whose work-items are 32 bits
+  for (long long r = 0; r < rows; r += MOST) {
+    const int n = (int)(rows - r < MOST ? rows - r : MOST);
+    hipLaunchKernelGGL((quantize_rows_dyn_kernel<BF16, F8, NW, KEEP>), dim3((unsigned)((n + ROWS - 1) / ROWS)),
+                       dim3(THREADS), 0, s, (const char*)x + (size_t)r * ldx * (BF16 ? 2 : 4), n, cols, ldx,
+                       q + (size_t)r * ldq, ldq, scale + r);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 template <bool BF16, bool F8>
-void launch_quantize(const void* x, int rows, int cols, int ldx, uint8_t* q, int ldq, float* scale, hipStream_t s) {
-  if (cols <= 2048)
-    hipLaunchKernelGGL((quantize_rows_dyn_kernel<BF16, F8, 1, 2048>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s,
-                       x, rows, cols, ldx, q, ldq, scale);
-  else if (cols <= 8192)
-    hipLaunchKernelGGL((quantize_rows_dyn_kernel<BF16, F8, 4, 8192>), dim3((unsigned)rows), dim3(256), 0, s, x, rows,
-                       cols, ldx, q, ldq, scale);
-  else if (cols <= 16384)
-    hipLaunchKernelGGL((quantize_rows_dyn_kernel<BF16, F8, 4, 16384>), dim3((unsigned)rows), dim3(256), 0, s, x, rows,
-                       cols, ldx, q, ldq, scale);
-  else
-    hipLaunchKernelGGL((quantize_rows_dyn_kernel<BF16, F8, 16, 65536>), dim3((unsigned)rows), dim3(1024), 0, s, x, rows,
-                       cols, ldx, q, ldq, scale);
+hipError_t launch_quantize(const void* x, int rows, int cols, int ldx, uint8_t* q, int ldq, float* scale,
+                           hipStream_t s) {
+  if (cols <= 2048) return launch_as<BF16, F8, 1, 2048>(x, rows, cols, ldx, q, ldq, scale, s);
+  if (cols <= 8192) return launch_as<BF16, F8, 4, 8192>(x, rows, cols, ldx, q, ldq, scale, s);
+  if (cols <= 16384) return launch_as<BF16, F8, 4, 16384>(x, rows, cols, ldx, q, ldq, scale, s);
+  return launch_as<BF16, F8, 16, 65536>(x, rows, cols, ldx, q, ldq, scale, s);
 }
 
 template <bool F8>
@@ -169,15 +177,12 @@ int quantize_rows_dyn(const void* x, int x_type, int rows, int cols, int ldx, ui
   if (x_type != DLQ_T_F32 && x_type != DLQ_T_BF16) return fail(DLQ_ERR_ARG, "quantize_rows_dyn: bad x_type");
   if (ldx < cols || ldq < cols) return fail(DLQ_ERR_ARG, "quantize_rows_dyn: row stride below cols");
   if (rows == 0) return DLQ_OK;
-  if (!grid_fits(rows, 1024)) return fail(DLQ_ERR_ARG, "quantize_rows_dyn: too many rows");
   if (!x || !q || !scale) return fail(DLQ_ERR_ARG, "quantize_rows_dyn: null pointer");
   if ((uintptr_t)x % (x_type == DLQ_T_BF16 ? 2 : 4) || (uintptr_t)scale % 4)
     return fail(DLQ_ERR_ARG, "quantize_rows_dyn: pointer not aligned to its element type");
-  if (x_type == DLQ_T_BF16)
-    launch_quantize<true, F8>(x, rows, cols, ldx, q, ldq, scale, (hipStream_t)stream);
-  else
-    launch_quantize<false, F8>(x, rows, cols, ldx, q, ldq, scale, (hipStream_t)stream);
-  const hipError_t e = hipGetLastError();
+  const hipError_t e = x_type == DLQ_T_BF16
+                           ? launch_quantize<true, F8>(x, rows, cols, ldx, q, ldq, scale, (hipStream_t)stream)
+                           : launch_quantize<false, F8>(x, rows, cols, ldx, q, ldq, scale, (hipStream_t)stream);
   return e == hipSuccess ? DLQ_OK
                          : fail(DLQ_ERR_LAUNCH, std::string("quantize_rows_dyn launch: ") + hipGetErrorString(e));
 }

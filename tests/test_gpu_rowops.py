@@ -437,6 +437,30 @@ def test_quantize_rows_dyn_longest_rows(gpu, t, cols, ld):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("t", ["s8", "f8"])
+@pytest.mark.parametrize("rows,cols", [((1 << 22) + 5, 7), ((1 << 26) - 1, 1), ((1 << 22) + 1, 2050)])
+def test_quantize_rows_dyn_many_rows(gpu, t, rows, cols):
+    """More rows than one launch takes."""
+    from dlq_amd import ops
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    r = torch.arange(rows, device="cuda", dtype=torch.int32)
+    x.copy_(((r % 1013) + 1)[:, None])
+    x[:, -1] = -((r % 1021) + 1).bfloat16()
+    q, s = (ops.quantize_rows_dyn_s8 if t == "s8" else ops.quantize_rows_dyn_f8)(x)
+    del r
+    m = 127.0 if t == "s8" else 448.0
+    for c in range(0, rows, 1 << 22):
+        v = x[c:c + (1 << 22)].float()
+        scale = v.abs().amax(1) / torch.tensor(m, device="cuda")
+        assert torch.equal(s[c:c + (1 << 22)], scale)
+        v = (v * (torch.ones_like(scale) / scale)[:, None]).clamp(-m, m)
+        want = v.round().to(torch.int8) if t == "s8" else v.to(F8).view(torch.uint8)
+        assert torch.equal(q[c:c + (1 << 22)], want)
+        del v, scale, want
+    del x, q, s
+    torch.cuda.empty_cache()
+
+
 # -------------------------------------------------------- log probabilities
 
 def lp_bounds(x):
