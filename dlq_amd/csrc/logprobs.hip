@@ -630,9 +630,8 @@ __global__ __launch_bounds__(256, 8) void logprobs_join_kernel(const LogprobArgs
 // a row in one wave's registers, in a workgroup's, or in chunks of the latter
 int chunks_of(int K) { return K <= kWaveChunk ? 1 : (K - 1) / kGroupChunk + 1; }
 
-
 template <bool BF16>
-hipError_t launch_logprobs(const LogprobArgs& a, int rows, hipStream_t s) {
+hipError_t launch_rows(const LogprobArgs& a, int rows, hipStream_t s) {
   const dim3 threads(256);
   if (a.chunks > 1) {
     hipLaunchKernelGGL(logprobs_chunk_kernel<BF16>, dim3((unsigned)rows * (unsigned)a.chunks), threads, 0, s, a);
@@ -653,6 +652,32 @@ hipError_t launch_logprobs(const LogprobArgs& a, int rows, hipStream_t s) {
       hipLaunchKernelGGL((logprobs_row_kernel<BF16, 4, kLane>), grid, threads, 0, s, a, rows);
   }
   return hipGetLastError();
+}
+
+template <bool BF16>
+hipError_t launch_logprobs(const LogprobArgs& all, int rows, hipStream_t s) {
+  // rows of one launch, whose work-items are 32 bits: 2^22 workgroups at most
+  const long long most = (1 << 22) / all.chunks;
+  for (long long r = 0; r < rows; r += most) {
+    LogprobArgs a = all;
+    a.x = (const char*)a.x + (size_t)r * a.ldx * (BF16 ? 2 : 4);
+    if (a.tokens) {
+      a.tokens += r;
+      a.logprob += r;
+    }
+    if (a.entropy) a.entropy += r;
+    if (a.top) {
+      a.top_idx += r * a.top;
+      a.top_logprob += r * a.top;
+    }
+    if (a.chunks > 1) {
+      a.heads += r * a.chunks * 64;
+      a.parts += r * a.chunks * 4;
+    }
+    const hipError_t e = launch_rows<BF16>(a, (int)(rows - r < most ? rows - r : most), s);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
@@ -683,7 +708,6 @@ int dlq_logprobs(const void* x, int x_type, int rows, int K, int ldx, const int3
     return fail(DLQ_ERR_ARG, "logprobs: pointer not aligned to its element type");
   const int chunks = chunks_of(K);
   LogprobArgs a = {x, K, ldx, top, chunks, tokens, logprob, entropy, top_idx, top_logprob, nullptr, nullptr};
-  if (!grid_fits((long long)rows * a.chunks, 256)) return fail(DLQ_ERR_ARG, "logprobs: too many rows");
   const size_t need = dlq_logprobs_workspace_bytes(rows, K, top);
   if (need && (!workspace || ws_bytes < need || (uintptr_t)workspace % 8))
     return fail(DLQ_ERR_ARG, "logprobs: workspace missing, too small or not 8-byte aligned");

@@ -635,6 +635,50 @@ def test_logprobs_offsets_past_32_bits(gpu):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("rows,K", [((1 << 24) + 3, 2), ((1 << 22) + 9, 70), ((1 << 22) + 1, 2050), ((1 << 21) + 3, 8193)])
+def test_logprobs_many_rows(gpu, rows, K):
+    """More rows than one launch takes: a 5 somewhere in a row of zeros."""
+    from dlq_amd import ops
+    x = torch.zeros(rows, K, dtype=torch.bfloat16, device="cuda")
+    at = (torch.arange(rows, device="cuda") * 37) % K
+    x.scatter_(1, at[:, None], 5.0)
+    tokens = torch.where(at % 3 == 0, at, (at + 1) % K).int()
+    r = ops.logprobs(x, tokens, 2)
+    S = math.exp(5) + K - 1
+    lp = (5 - math.log(S), -math.log(S))
+    H = -(math.exp(5) / S * lp[0] + (K - 1) / S * lp[1])
+    tol = U * (K / 64 + 64 + 40) * (1 + abs(lp[1]) + 5)  # terms of S and T, and the logarithm's and quotient's roundings
+    second = torch.where(at == 0, 1, 0)
+    assert torch.equal(r.top_idx[:, 0], at.int()) and torch.equal(r.top_idx[:, 1], second.int())
+    for got, want in ((r.logprob, torch.where(tokens == at, lp[0], lp[1])), (r.entropy, H),
+                      (r.top_logprob[:, 0], lp[0]), (r.top_logprob[:, 1], lp[1])):
+        assert float((got.double() - want).abs().max()) <= tol
+    del x
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("top", [0, 3, 6])
+def test_logprobs_longest_row(gpu, top):
+    """2^31 - 1 logits, zeros but for three."""
+    from dlq_amd import ops
+    K = 2 ** 31 - 1
+    x = torch.zeros(1, K, dtype=torch.bfloat16, device="cuda")
+    x[0, 5], x[0, K - 1], x[0, 2 ** 30] = 3.0, 4.0, 2.0
+    r = ops.logprobs(x, torch.tensor([K - 1], dtype=torch.int32, device="cuda"), top)
+    S = math.exp(3) + math.exp(4) + math.exp(2) + K - 3
+    ls = math.log(S)
+    H = ls - (3 * math.exp(3) + 4 * math.exp(4) + 2 * math.exp(2)) / S
+    # a sum: 32 logits of a lane, a wave's lanes, a thread's 4096 parts, the workgroup's
+    tol = U * (32 + 6 + 4096 + 10 + 40) * (1 + ls)
+    assert abs(r.entropy.item() - H) <= tol and abs(r.logprob.item() - (4 - ls)) <= tol
+    if top:
+        assert r.top_idx[0].tolist() == [K - 1, 5, 2 ** 30, 0, 1, 2][:top]
+        want = torch.tensor([4.0, 3, 2, 0, 0, 0][:top], dtype=torch.float64) - ls
+        assert float((r.top_logprob[0].double().cpu() - want).abs().max()) <= tol
+    del x
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------- together, streams, graphs
 
 def make_layer(seed, t, d, h, E, V):
