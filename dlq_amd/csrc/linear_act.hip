@@ -25,6 +25,7 @@ struct LinearArgs {
   size_t ldx, ldw, ldy, ldr;
   int odd;             // some row of x or w does not start on a dword
   int act, bf16, vec;  // vec: y, res, ws and bias take aligned 4-element accesses
+  int cut;             // e4m3: the fp8 matrix instructions may be taken
   int E;               // 0: one product over all rows
   const int* off;      // [E + 1], E > 0
 };
@@ -165,10 +166,11 @@ __device__ __forceinline__ bool expert_tile(const LinearArgs& a, int t, int& e, 
 // e4m3: the fp8 forms of the matrix pipe bring the products of 8 consecutive K
 // to the largest one's exponent and cut them 13 bits below it (measured: a
 // product of 2^2 beside one of 2^16 is lost, 1.5 * 2^3 keeps 2^3), which is
-// coarser than a 32-bit sum.  The codes are bf16 values as well, so here they
+// coarser than a 32-bit sum: 1.4e-5 of a result on normal data, all of it where
+// a row's large products cancel.  The codes are bf16 values as well, so they
 // are widened (one conversion per two codes) and multiplied as bf16, whose
-// products are exact and sums fp32: twice the matrix instructions, in a kernel
-// that waits for memory.
+// products are exact and sums fp32.  Here that is twice the matrix
+// instructions in a kernel that waits for memory; for the tiles see below.
 template <bool F8>
 struct Mma {
   typedef v4i frag;
@@ -386,15 +388,18 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
 // the 256 KB that LDS moves in a stage's 2048 matrix cycles (with 128 x 64
 // per wave: 256 KB, the bound).  8192^3, bf16 out: int8 495 us, 2.22 POPS, the
 // clock at 1.7 GHz by the power limit and the matrix unit busy 55 % of the
-// cycles; e4m3 440 us, 2.5 PFLOP/s.  Waves of 64 x 64 (128 x 128 tiles) read
+// cycles.  Waves of 64 x 64 (128 x 128 tiles) read
 // LDS for as long as they multiply: 576 us.  The small tiles are bound by what
 // a stage takes from DMA to barrier, so they have more slots and up to 128
 // bytes of K per fragment step.
 //
-// e4m3 here uses the fp8 matrix instructions, whose cut products (see Mma) are
-// off by up to 7 * 2^-13 of the largest of each 8: 1.4e-5 of the result on
-// normal data, which bf16's rounding (2^-9) hides; only bf16 outputs come here.
-template <bool F8, int NV>
+// e4m3 is widened to bf16 here as well (see Mma), behind the LDS read and while
+// matrix instructions run that do not need the fragment: twice the matrix
+// cycles per code, so 8192^3 takes 765 us, 1.44 PFLOP/s, what a bf16 product
+// of this size reaches.  kF8Cut (the caller's DLQ_FP8_SUMS) takes the fp8
+// instructions, 440 us, and their cut products.
+enum { kS8, kF8, kF8Cut };
+template <int T, int NV>
 struct TileMma {  // a fragment: NV 16-byte reads, 32 K bytes of a row each
   typedef v16i acc_t;
   typedef v4i sum4;
@@ -405,7 +410,17 @@ struct TileMma {  // a fragment: NV 16-byte reads, 32 K bytes of a row each
   }
 };
 template <int NV>
-struct TileMma<true, NV> {
+struct TileMma<kF8, NV> {
+  typedef v16f acc_t;
+  typedef v4f sum4;
+  typedef Mma<true>::frag wide;  // 16 codes as bf16
+  static __device__ __forceinline__ v16f go(const wide& a, const wide& b, v16f c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h[0], b.h[0], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h[1], b.h[1], c, 0, 0, 0);
+  }
+};
+template <int NV>
+struct TileMma<kF8Cut, NV> {
   static_assert(NV % 2 == 0, "64 K bytes per instruction");
   typedef v16f acc_t;
   typedef v4f sum4;
@@ -439,9 +454,9 @@ struct TileLds {
 };
 
 // Columns from n0 on of rows [m0, m1) of expert e.
-template <bool F8, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, bool RES>
+template <int T, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, bool RES>
 __device__ __forceinline__ void linear_tile(const LinearArgs& a, int e, int m0, int m1, int n0, int8_t* lds) {
-  typedef TileMma<F8, NV> MM;
+  typedef TileMma<T, NV> MM;
   typedef typename MM::acc_t acc_t;
   typedef typename MM::sum4 sum4;
   constexpr int NW = WN * WM, TN = 32 * WN * NI, TM = 32 * WM * MJ;
@@ -533,6 +548,11 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a, int e, int m0, 
     else
       fw[b][f - MJ][v] = *(const v4i*)(p + ((wn * NI + f - MJ) * 32 + lr) * KB);
   };
+  // e4m3 widened: the w fragment in use and the next, the x fragments of a step.
+  // What comes next is widened while matrix instructions run that do not need it.
+  typedef Mma<true> Wide;
+  Wide::frag cw[2][NV], cx[MJ][NV];
+  static_assert(NI == 1 || NI % 2 == 0, "a step starts with cw[0]");
   // one step's matrix instructions on buffer b; between them, in its first
   // half, the reads of the next step (rslot >= 0), and DMA pieces of stage dst
   // (dst >= 0)
@@ -546,8 +566,25 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a, int e, int m0, 
           if (q * NM / (2 * NR) == t) read(rslot, rstep, b ^ 1, q);
       }
       __builtin_amdgcn_sched_barrier(0);
-      acc[i][j] = MM::go(fw[b][i], fx[b][j], acc[i][j]);
-      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (T == kF8) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          if (NM == 1) {  // a step is too short to wait for the next one's reads in it
+            cw[0][v] = Wide::prep(fw[b][0][v]);
+            cx[0][v] = Wide::prep(fx[b][0][v]);
+          }
+          acc[i][j] = MM::go(cw[i & 1][v], cx[j][v], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (NM == 1) continue;
+          if (i + 1 == NI && rslot >= 0) cx[j][v] = Wide::prep(fx[b ^ 1][j][v]);
+          if (j + 1 == MJ && i + 1 < NI) cw[(i + 1) & 1][v] = Wide::prep(fw[b][i + 1][v]);
+          if (t + 1 == NM && rslot >= 0) cw[0][v] = Wide::prep(fw[b ^ 1][0][v]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        acc[i][j] = MM::go(fw[b][i], fx[b][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       if (dst >= 0) {
 #pragma unroll
         for (int r = 0; r < PP; ++r)
@@ -614,6 +651,14 @@ __device__ __forceinline__ void linear_tile(const LinearArgs& a, int e, int m0, 
   if (nst > 0) {
 #pragma unroll
     for (int q = 0; q < NR; ++q) read(0, 0, 0, q);
+    if constexpr (T == kF8 && NM > 1) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        cw[0][v] = Wide::prep(fw[0][0][v]);
+#pragma unroll
+        for (int j = 0; j < MJ; ++j) cx[j][v] = Wide::prep(fx[0][j][v]);
+      }
+    }
     int s = 0, slot = 0;
     const auto after = [](int k) { return k + 1 == SLOTS ? 0 : k + 1; };
     // two stages at a time where a stage is an odd number of steps or goes
@@ -791,20 +836,30 @@ __device__ __forceinline__ bool tile_at(const LinearArgs& a, int l, int nbm, int
   return true;
 }
 
-template <bool F8, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE, bool RES>
+template <int T, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE, bool RES>
 __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const LinearArgs a, int nbm, int nbn) {
   __shared__ __attribute__((aligned(16))) int8_t lds[TileLds<WN, WM, NI, MJ, KB, SLOTS, RES>::BYTES];
   int e, m0, m1, n0;  // each XCD takes a run of tiles
   if (!tile_at<32 * WN * NI, 32 * WM * MJ>(a, xcd_remap(blockIdx.x, gridDim.x), nbm, nbn, e, m0, m1, n0)) return;
-  linear_tile<F8, REG, WN, WM, NI, MJ, NV, KB, SLOTS, RES>(a, e, m0, m1, n0, lds);
+  linear_tile<T, REG, WN, WM, NI, MJ, NV, KB, SLOTS, RES>(a, e, m0, m1, n0, lds);
 }
+
+// 16-byte reads per fragment.  Widened e4m3 has the shortest in the large tiles:
+// its widening runs behind more matrix instructions then, and spills nothing
+// (8192^3: 760 us, 1020 with two; 128 x 128 tiles of 4096^3 143, 147 with two).
+template <int T>
+constexpr int kNv64 = T == kF8Cut ? 2 : 4;
+template <int T>
+constexpr int kNvReg64 = T == kF8 ? 2 : 4;
+template <int T, int WIDE>
+constexpr int kNv = T == kF8 ? 1 : WIDE;
 
 // 256 x 256 tiles, from the `whole`-th on in four workgroups of 128 x 128, which
 // start as CUs come free: a last round that would leave most of them idle takes
-// a third of the time.  16384 rows over 8 experts of 4096 x 4096 e4m3 318 -> 288
-// us, 4096 x 5120 x 16384 int8 335 -> 292, 4096 x 4608 x 4096 96 -> 87 (as a
-// launch behind the first one it gained nothing: that waits for the slowest).
-template <bool F8, bool RES>
+// a third of the time.  int8: 4096 x 5120 x 16384 335 -> 292 us, 4096 x 4608 x
+// 4096 96 -> 87 (as a launch behind the first one it gained nothing: that waits
+// for the slowest).
+template <int T, bool RES>
 __global__ __launch_bounds__(256, 1) void linear_tile_quarters_kernel(const LinearArgs a, int nbm, int nbn, int whole) {
   constexpr int B0 = TileLds<2, 2, 4, 4, 128, 2, RES>::BYTES, B1 = TileLds<2, 2, 2, 2, 128, 4, RES>::BYTES;
   __shared__ __attribute__((aligned(16))) int8_t lds[B0 > B1 ? B0 : B1];
@@ -812,14 +867,14 @@ __global__ __launch_bounds__(256, 1) void linear_tile_quarters_kernel(const Line
   const int b = blockIdx.x;
   if (b < whole) {
     if (!tile_at<256, 256>(a, xcd_remap(b, whole), nbm, nbn, e, m0, m1, n0)) return;
-    linear_tile<F8, false, 2, 2, 4, 4, 2, 128, 2, RES>(a, e, m0, m1, n0, lds);
+    linear_tile<T, false, 2, 2, 4, 4, kNv<T, 2>, 128, 2, RES>(a, e, m0, m1, n0, lds);
   } else {
     const int q = b - whole;
     if (!tile_at<256, 256>(a, whole + q / 4, nbm, nbn, e, m0, m1, n0)) return;
     m0 += q % 2 * 128;
     n0 += q / 2 % 2 * 128;
     if (m0 >= m1 || n0 >= a.N) return;
-    linear_tile<F8, false, 2, 2, 2, 2, 4, 128, 4, RES>(a, e, m0, m1, n0, lds);
+    linear_tile<T, false, 2, 2, 2, 2, kNv<T, 4>, 128, 4, RES>(a, e, m0, m1, n0, lds);
   }
 }
 
@@ -831,17 +886,17 @@ long row_tiles(const LinearArgs& a, int BM) {
   return t < a.M ? t : a.M;
 }
 
-template <bool F8, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE>
+template <int T, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE>
 hipError_t launch_tile(const LinearArgs& a, hipStream_t s) {
   constexpr int TN = 32 * WN * NI, TM = 32 * WM * MJ;
   const long nbn = (a.N + TN - 1) / TN, nbm = row_tiles(a, TM);
   if (!grid_fits(nbm * nbn, WN * WM * 64)) return hipErrorInvalidValue;
   const dim3 grid((unsigned)(nbm * nbn)), threads(WN * WM * 64);
   if (a.vec && a.res)
-    hipLaunchKernelGGL((linear_tile_kernel<F8, REG, WN, WM, NI, MJ, NV, KB, SLOTS, WPE, true>), grid, threads, 0, s, a,
+    hipLaunchKernelGGL((linear_tile_kernel<T, REG, WN, WM, NI, MJ, NV, KB, SLOTS, WPE, true>), grid, threads, 0, s, a,
                        (int)nbm, (int)nbn);
   else
-    hipLaunchKernelGGL((linear_tile_kernel<F8, REG, WN, WM, NI, MJ, NV, KB, SLOTS, WPE, false>), grid, threads, 0, s, a,
+    hipLaunchKernelGGL((linear_tile_kernel<T, REG, WN, WM, NI, MJ, NV, KB, SLOTS, WPE, false>), grid, threads, 0, s, a,
                        (int)nbm, (int)nbn);
   return hipGetLastError();
 }
@@ -869,7 +924,8 @@ int num_cus() {
 }
 
 // Which kernel.  us on one MI355X, weights from memory, 16-byte rows (int8; e4m3
-// within 10 %, 256 x 256 up to 15 % faster); then K odd, through registers.
+// by the fp8 instructions within 10 %, 256 x 256 up to 15 % faster); then K odd,
+// through registers.
 //                        direct            tiles
 //   M x N x K            16    32    64    64    128/4  128/2  256
 //   1 x 4096 x 4096     5.8   8.8    15    12     21     33     55
@@ -890,6 +946,22 @@ int num_cus() {
 //   256 x 4096 x 4099    88    51    33    28     37
 //   1003 x 5000 x 2737  247   151   101    62     58
 //   4096 x 4096 x 4099 1316   721   483   229    174
+// e4m3 widened:          16    32    64    64    128/4  128/2  256
+//   16 x 4096 x 4096    7.3   9.6    20    16     34     33     90
+//   32 x 4096 x 4096     11    11    21    16     34     33     90
+//   32 x 12288 x 4096    25    18    20    16     34     33     89
+//   64 x 4096 x 4096     17    11    23    16     35     34     92
+//   256 x 4096 x 4096    60    32    22    17     35     34     95
+//   512 x 4096 x 4096   115    61    42    25     37     34     93
+//   1003 x 5000 x 2736  133    84    70    49     56     42     80
+//   2276 x 953 x 16128  473   255   206   113    119    117    339
+//   2048 x 4096 x 4096  453   229   165    92     78     61     96
+//   4096 x 4096 x 4096  902   456   322   177    153    122    111
+//   K odd:                                 64   128 x 64
+//   64 x 4096 x 4099     27    19    37    28     39
+//   256 x 4096 x 4099    85    50    34    28     37
+//   1003 x 5000 x 2737  246   140   109    62     62
+//   4096 x 4096 x 4099 1343   774   511   249    212
 // A tile's stage costs what its loads and its chain of steps take, nearly the
 // same whatever else runs: so the tiles are compared by rounds of workgroups
 // times a round's cost (us per 1024 of K with one and with two workgroups on a
@@ -898,11 +970,16 @@ struct TileCost {
   int tn, tm, per_cu;
   float one, two, fixed;
 };
-template <bool F8>
+template <int T>
 constexpr TileCost kDmaTiles[4] = {{64, 64, 2, 2.0f, 3.3f, 2.5f},   // 64 x 64, 5 slots
                                    {128, 128, 1, 4.5f, 5.2f, 5.f},  // 128 x 128, 4 slots
                                    {128, 128, 2, 5.0f, 9.0f, 4.f},  // 128 x 128, 2 slots
-                                   {256, 256, 1, F8 ? 13.5f : 15.f, F8 ? 13.5f : 15.f, 9.f}};  // 256 x 256, 2 slots
+                                   {256, 256, 1, T == kS8 ? 15.f : 13.5f, T == kS8 ? 15.f : 13.5f, 9.f}};  // 256 x 256, 2 slots
+template <>
+constexpr TileCost kDmaTiles<kF8>[4] = {{64, 64, 2, 2.5f, 4.5f, 4.5f},
+                                        {128, 128, 1, 6.9f, 6.9f, 7.f},
+                                        {128, 128, 2, 6.6f, 12.2f, 7.f},
+                                        {256, 256, 1, 21.7f, 21.7f, 15.f}};
 constexpr TileCost kRegTiles[2] = {{64, 64, 2, 5.6f, 7.0f, 4.f}, {128, 64, 2, 8.0f, 9.9f, 5.f}};
 
 // rows' tiles of height tm; grouped: as if each expert's last one were half full
@@ -946,34 +1023,35 @@ int best_tile(const LinearArgs& a, const TileCost (&tiles)[N], int& whole) {
   return best;
 }
 
-template <bool F8>
+template <int T>
 hipError_t launch_quarters(const LinearArgs& a, int whole, hipStream_t s) {
   const long nbn = (a.N + 255) / 256, nbm = row_tiles(a, 256);
   if (whole > nbm * nbn) whole = (int)(nbm * nbn);
   const long grid = whole + 4 * (nbm * nbn - whole);
   if (!grid_fits(grid, 256)) return hipErrorInvalidValue;
   if (a.vec && a.res)
-    hipLaunchKernelGGL((linear_tile_quarters_kernel<F8, true>), dim3((unsigned)grid), dim3(256), 0, s, a, (int)nbm,
+    hipLaunchKernelGGL((linear_tile_quarters_kernel<T, true>), dim3((unsigned)grid), dim3(256), 0, s, a, (int)nbm,
                        (int)nbn, whole);
   else
-    hipLaunchKernelGGL((linear_tile_quarters_kernel<F8, false>), dim3((unsigned)grid), dim3(256), 0, s, a, (int)nbm,
+    hipLaunchKernelGGL((linear_tile_quarters_kernel<T, false>), dim3((unsigned)grid), dim3(256), 0, s, a, (int)nbm,
                        (int)nbn, whole);
   return hipGetLastError();
 }
 
-template <bool F8>
+template <int T>
 hipError_t launch_best_tile(const LinearArgs& a, bool dma, hipStream_t s) {
   int whole;
   if (!dma) {
-    if (best_tile(a, kRegTiles, whole) == 0) return launch_tile<F8, true, 2, 2, 1, 1, 4, 128, 2, 2>(a, s);
-    return launch_tile<F8, true, 2, 2, 2, 1, 2, 128, 2, 2>(a, s);
+    if (best_tile(a, kRegTiles, whole) == 0) return launch_tile<T, true, 2, 2, 1, 1, kNvReg64<T>, 128, 2, 2>(a, s);
+    return launch_tile<T, true, 2, 2, 2, 1, 2, 128, 2, 2>(a, s);
   }
-  switch (best_tile(a, kDmaTiles<F8>, whole)) {
-    case 0: return launch_tile<F8, false, 2, 2, 1, 1, F8 ? 2 : 4, 128, 5, 2>(a, s);
-    case 1: return launch_tile<F8, false, 2, 2, 2, 2, 4, 128, 4, 1>(a, s);
-    case 2: return launch_tile<F8, false, 2, 2, 2, 2, 2, 128, 2, 2>(a, s);
+  switch (best_tile(a, kDmaTiles<T>, whole)) {
+    case 0: return launch_tile<T, false, 2, 2, 1, 1, kNv64<T>, 128, 5, 2>(a, s);
+    case 1: return launch_tile<T, false, 2, 2, 2, 2, kNv<T, 4>, 128, 4, 1>(a, s);
+    case 2: return launch_tile<T, false, 2, 2, 2, 2, kNv<T, 2>, 128, 2, 2>(a, s);
     default:
-      return whole > 0 ? launch_quarters<F8>(a, whole, s) : launch_tile<F8, false, 2, 2, 4, 4, 2, 128, 2, 1>(a, s);
+      return whole > 0 ? launch_quarters<T>(a, whole, s)
+                       : launch_tile<T, false, 2, 2, 4, 4, kNv<T, 2>, 128, 2, 1>(a, s);
   }
 }
 
@@ -988,9 +1066,10 @@ hipError_t launch_linear_any(const LinearArgs& a, bool dma, hipStream_t s) {
   const float cus = (float)num_cus();
   const auto wgs = [&](int t) { return tiles_of_rows(a, t) * (float)((a.N + t - 1) / t); };
   // tiles from half as many workgroups as CUs on; their rows' byte offsets are 32 bits
-  if (rows > 16.f && wgs(64) >= 0.5f * cus && (!F8 || a.bf16) && a.ldx <= (1 << 22) && a.ldw <= (1 << 22) &&
-      a.ldr <= (1 << 21))
-    return launch_best_tile<F8>(a, dma, s);
+  if (rows > 16.f && wgs(64) >= 0.5f * cus && a.ldx <= (1 << 22) && a.ldw <= (1 << 22) && a.ldr <= (1 << 21)) {
+    if constexpr (!F8) return launch_best_tile<kS8>(a, dma, s);
+    return a.cut ? launch_best_tile<kF8Cut>(a, dma, s) : launch_best_tile<kF8>(a, dma, s);
+  }
   if (rows <= 16.f || wgs(16) <= 2.f * cus)
     return a.K < 8192 ? launch_direct<F8, 1, 1, 4, 4>(a, s) : launch_direct<F8, 1, 1, 8, 4>(a, s);
   return wgs(64) < cus ? launch_direct<F8, 2, 2, 4, 4>(a, s) : launch_direct<F8, 4, 4, 4, 2>(a, s);
@@ -1002,7 +1081,8 @@ int linear_any(const char* who, const dlq_linear_desc* d, int E, const int32_t* 
   const auto bad = [&](const char* what) { return fail(DLQ_ERR_ARG, std::string(who) + ": " + what); };
   if (!d || d->M < 0 || d->N < 0 || d->K < 0) return bad("bad shape");
   if (d->K > 131071) return bad("K above 131071");
-  if (d->act < DLQ_ACT_NONE || d->act > DLQ_ACT_SILU) return bad("bad act");
+  const int act = F8 ? d->act & ~DLQ_FP8_SUMS : d->act;
+  if (act < DLQ_ACT_NONE || act > DLQ_ACT_SILU) return bad("bad act");
   if (d->out_type != DLQ_T_F32 && d->out_type != DLQ_T_BF16) return bad("bad out_type");
   if (d->ldx < d->K || d->ldw < d->K) return bad("row stride below K");
   if (d->ldy < d->N || (res && d->ldr < d->N)) return bad("row stride below N");
@@ -1028,7 +1108,8 @@ int linear_any(const char* who, const dlq_linear_desc* d, int E, const int32_t* 
   a.ldw = d->ldw;
   a.ldy = d->ldy;
   a.ldr = res ? d->ldr : 0;
-  a.act = d->act;
+  a.act = act;
+  a.cut = act != d->act;
   a.bf16 = d->out_type == DLQ_T_BF16;
   a.vec = ((uintptr_t)ws | (uintptr_t)bias) % 16 == 0 && ((uintptr_t)y | (uintptr_t)res) % (4 * es) == 0 &&
           d->N % 4 == 0 && d->ldy % 4 == 0 && (!res || d->ldr % 4 == 0);

@@ -24,6 +24,7 @@ DLQ_OUT_S8, DLQ_OUT_F32, DLQ_OUT_S32 = 0, 1, 2
 DLQ_PREC_INT8, DLQ_PREC_FP8 = 0, 1
 DLQ_T_F32, DLQ_T_BF16 = 0, 1
 DLQ_ACT = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+DLQ_FP8_SUMS = 256
 # kernel families of dlq_resnet18_timing (include/dlq.h DLQ_FAM_*)
 # (the first word names the int8 forward's kernel; the fp8 forward runs
 # stem_fused_kernel and block_l1_kernel in families 0 and 1)

@@ -18,8 +18,8 @@ from typing import NamedTuple
 import numpy as np
 import torch
 
-from .lib import (DLQ_ACT, DLQ_OUT_F32, DLQ_OUT_S8, DLQ_OUT_S32, DLQ_T_BF16, DLQ_T_F32, ConvDesc, LinearDesc,
-                  check, lib, ptr, raw_stream, stream_handle)
+from .lib import (DLQ_ACT, DLQ_FP8_SUMS, DLQ_OUT_F32, DLQ_OUT_S8, DLQ_OUT_S32, DLQ_T_BF16, DLQ_T_F32, ConvDesc,
+                  LinearDesc, check, lib, ptr, raw_stream, stream_handle)
 
 
 def out_dim(n, k, s, p):
@@ -538,10 +538,13 @@ def quantize_rows_dyn_f8(x: torch.Tensor, ld: int | None = None):
     return _quantize_rows_dyn("quantize_rows_dyn_f8", lib.dlq_quantize_rows_dyn_f8, torch.uint8, x, ld)
 
 
-def _linear(what, fn, code, x, w, x_scale, w_scale, bias, act, residual, out_dtype, out, offsets=None):
+def _linear(what, fn, code, x, w, x_scale, w_scale, bias, act, residual, out_dtype, out, offsets=None,
+            fp8_sums=False):
     kind = DLQ_ACT.get(act)
     if kind is None:
         raise ValueError(f"act must be one of {sorted(DLQ_ACT)}, got {act!r}")
+    if fp8_sums:
+        kind |= DLQ_FP8_SUMS
     if out is not None:
         out_dtype = out.dtype
     if out_dtype not in _TYPES:
@@ -594,10 +597,14 @@ def linear_act_s8(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None
 
 def linear_act_f8(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None, w_scale: torch.Tensor,
                   bias: torch.Tensor | None = None, act: str = "none", residual: torch.Tensor | None = None,
-                  out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
-    """e4m3 twin of linear_act_s8 (uint8 codes)."""
+                  out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
+                  fp8_sums: bool = False) -> torch.Tensor:
+    """e4m3 twin of linear_act_s8 (uint8 codes): exact products summed in fp32.
+    fp8_sums: larger products may take the fp8 matrix instructions, which are
+    faster and cut the products of 8 consecutive k 13 bits below the largest
+    of them (DLQ_FP8_SUMS)."""
     return _linear("linear_act_f8", lib.dlq_linear_act_f8, torch.uint8, x, w, x_scale, w_scale, bias, act, residual,
-                   out_dtype, out)
+                   out_dtype, out, None, fp8_sums)
 
 
 def linear_grouped_s8(x: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None,
@@ -618,12 +625,12 @@ def linear_grouped_s8(x: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor, x
 def linear_grouped_f8(x: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor | None,
                       w_scale: torch.Tensor, bias: torch.Tensor | None = None, act: str = "none",
                       residual: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float32,
-                      out: torch.Tensor | None = None) -> torch.Tensor:
-    """e4m3 twin of linear_grouped_s8 (uint8 codes)."""
+                      out: torch.Tensor | None = None, fp8_sums: bool = False) -> torch.Tensor:
+    """e4m3 twin of linear_grouped_s8 (uint8 codes); fp8_sums: see linear_act_f8."""
     if offsets is None:
         raise TypeError("offsets is required")
     return _linear("linear_grouped_f8", lib.dlq_linear_grouped_f8, torch.uint8, x, w, x_scale, w_scale, bias, act,
-                   residual, out_dtype, out, offsets)
+                   residual, out_dtype, out, offsets, fp8_sums)
 
 
 class LogProbs(NamedTuple):

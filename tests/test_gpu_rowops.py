@@ -115,6 +115,60 @@ def test_linear_shapes(gpu, t, M, N, K, out):
     close(got, *product64(**c, act=act, out_dtype=out), f"{M}x{N}x{K}")
 
 
+def sums64(x, w, xs, ws, bias, act, res, out_dtype, cut=False):
+    """product64 of e4m3 codes with the bound of exact products and fp32 sums
+    whatever the output; cut: with the fp8 instructions' share."""
+    y, tol = product64(x, w, xs, ws, bias, act, res, torch.float32)
+    if cut:
+        g = [torch.nn.functional.pad(values(v).abs(), (0, -v.shape[1] % 8)).view(len(v), -1, 8).amax(2) for v in (x, w)]
+        tol = tol + 1.13 * 7 * 2.0 ** -13 * (g[0] @ g[1].T) * (1.0 if xs is None else xs.double()[:, None]) * ws.double()
+    return y, tol if out_dtype == torch.float32 else tol + HALF[out_dtype] * (y.abs() + tol)
+
+
+F8_SHAPES = [s for s in SHAPES if s[0] > 16] + [(40, 4100, 4096), (33, 8200, 1043), (1003, 5000, 2736)]
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("cut", [False, True], ids=["exact", "cut"])
+@pytest.mark.parametrize("M,N,K", F8_SHAPES)
+def test_linear_f8_sums(gpu, M, N, K, cut, out):
+    """Exact products and fp32 sums at every size, with bf16 output as well,
+    unless the caller allows the fp8 instructions."""
+    from dlq_amd import ops
+    rng = np.random.default_rng([M, N, K, 1])
+    c = case(rng, "f8", M, N, K, out, res=(M + N) % 2 == 0)
+    act = ACTS[(M + K) % 5]
+    got = ops.linear_act_f8(dev(c["x"]), dev(c["w"]), dev(c["xs"]), dev(c["ws"]), dev(c["bias"]), act, dev(c["res"]),
+                            out, fp8_sums=cut)
+    close(got, *sums64(**c, act=act, out_dtype=out, cut=cut), f"{M}x{N}x{K}")
+
+
+def cancelling(rng, M, N, K):
+    """e4m3 rows whose large values cancel: +-448 next to values 2^17 times smaller, weights +-1."""
+    x = torch.from_numpy(rng.choice([-1.0, 1.0], (M, K)).astype(np.float32)) * 2.0 ** -8
+    x[:, 0::16], x[:, 8::16] = 448.0, -448.0
+    w = torch.ones(N, K)
+    w[1::2, 1::2] = -1.0
+    return [v.to(F8).view(torch.uint8) for v in (x, w)]
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(5, 300, 512), (40, 12288, 512), (300, 1700, 512), (300, 1700, 528), (1100, 4100, 512),
+                                   (4100, 4500, 528), (300, 1700, 513)])
+def test_linear_f8_cancelling_products(gpu, M, N, K, out):
+    """Every partial sum is a multiple of 2^-8 below 2^15, so fp32 sums are exact in any order."""
+    from dlq_amd import ops
+    x, w = cancelling(np.random.default_rng(K), M, N, K)
+    want = values(x) @ values(w).T
+    got = ops.linear_act_f8(x.cuda(), w.cuda(), None, torch.ones(N, device="cuda"), out_dtype=out)
+    assert torch.equal(got.cpu().double(), want.to(out).double())
+    E = 3
+    off = torch.tensor([0, M // 2, M // 2, M], dtype=torch.int32, device="cuda")
+    got = ops.linear_grouped_f8(x.cuda(), off, w.cuda().expand(E, N, K).contiguous(), None,
+                                torch.ones(E, N, device="cuda"), out_dtype=out)
+    assert torch.equal(got.cpu().double(), want.to(out).double())
+
+
 @pytest.mark.parametrize("t", ["s8", "f8"])
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("bias,res,xs", [(0, 0, 0), (1, 0, 1), (0, 1, 1), (1, 1, 0)])

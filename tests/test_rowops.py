@@ -56,6 +56,18 @@ def test_linear_refuses_pointers(fn):
     assert linear(fn, desc(N=0, ldy=0), x=None, w=None, ws=None, y=None, grouped=g)[0] == 0
 
 
+@pytest.mark.parametrize("fn", FNS + GFNS)
+def test_fp8_sums_belong_to_e4m3(fn):
+    """The flag beside an activation: unknown to int8, no activation by itself."""
+    g = (2, P) if fn in GFNS else None
+    for act in (256, 256 + 4):
+        rc, msg = linear(fn, desc(act=act, M=0), grouped=g)
+        assert (rc == 1 and "bad act" in msg) if fn.endswith("s8") else rc == 0
+    for act in (256 + 5, 512, 512 + 256, -256):
+        rc, msg = linear(fn, desc(act=act, M=0), grouped=g)
+        assert rc == 1 and "bad act" in msg
+
+
 @pytest.mark.parametrize("fn", GFNS)
 def test_grouped_refuses(fn):
     rc, msg = linear(fn, desc(), grouped=(2, None))
