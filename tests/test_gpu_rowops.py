@@ -180,6 +180,32 @@ def test_linear_epilogue(gpu, t, act, bias, res, xs):
         close(got, *product64(**c, act=act, out_dtype=torch.float32))
 
 
+@pytest.mark.parametrize("M", [1, 40])
+def test_gelu_in_fp32(gpu, M):
+    """GELU of the bias (K = 0) over [-15, 15] against v Phi(v).  Near 0 it is
+    v (1/2 + v R): three roundings in v R (at most 0.4), the sum's and the
+    product's, 1.2 + 0.9 + 0.9 units of u |v|.  Beyond 1.25 max(v, 0) - |v| E
+    with E <= 0.11 off by at most 8 u of itself (Q <= 3.3 there and its fma
+    chain, the exponential's 2 u), a fit of 0.3 u and the last rounding:
+    0.9 + 0.3 + 1.  So 3 u |v| holds everywhere."""
+    from dlq_amd import ops
+    v = torch.cat([torch.linspace(-15, 15, 1 << 18), torch.linspace(-1.4, 1.4, 1 << 16), 10.0 ** torch.linspace(-30, 30, 500),
+                   -(10.0 ** torch.linspace(-30, 30, 500))])
+    N = v.numel()
+    y = ops.linear_act_s8(torch.zeros(M, 0, dtype=torch.int8, device="cuda"), torch.zeros(N, 0, dtype=torch.int8, device="cuda"),
+                          None, torch.ones(N, device="cuda"), v.cuda(), "gelu").double().cpu()
+    x = v.double()
+    want = x * torch.special.log_ndtr(x).exp()  # ndtr itself is 1 + erf, nothing below -8.3
+    close(y, want.expand(M, N), (3 * U * x.abs() + 1e-38).expand(M, N))
+    tail = (x < -1.25) & (x > -13)  # right in itself where 1 + erf would cancel
+    # the exponential has no subnormal results: an E below 2^-126 (|v| > 12.9) is 0
+    close(y[:, tail], want[tail].expand(M, -1), (2e-3 * want[tail].abs() + 2.0 ** -126 * x[tail].abs()).expand(M, -1))
+    ends = torch.tensor([0.0, -0.0, math.inf, -math.inf, math.nan, 1.25, -1.25, 3e38])
+    z = ops.linear_act_s8(torch.zeros(M, 0, dtype=torch.int8, device="cuda"), torch.zeros(8, 0, dtype=torch.int8, device="cuda"),
+                          None, torch.ones(8, device="cuda"), ends.cuda(), "gelu").cpu()[-1]
+    assert z[0] == 0 and z[1] == 0 and z[2] == math.inf and z[3] == 0 and z[4].isnan() and z[7] == ends[7]
+
+
 @pytest.mark.parametrize("t", ["s8", "f8"])
 @pytest.mark.parametrize("M,N,K", [(1, 100, 100), (9, 80, 333), (70, 200, 161), (200, 300, 160), (260, 520, 336)])
 @pytest.mark.parametrize("px,pw,py,pr", [(1, 3, 5, 7), (16, 16, 4, 4), (48, 0, 16, 0), (7, 16, 1, 8)])
