@@ -228,7 +228,8 @@ struct Mma<true> {
 // 20 MB by the latency of the loads: so each wave has 2 U of them in flight
 // (U steps ahead), what is left of a slice is loaded at once (8 x 1000 x 2000
 // 3.4 us; step by step 4.5), so are the epilogue's operands, behind the first
-// loads, and K is split until every CU has a workgroup.  int8, bf16
+// loads, and K is split over the waves of a workgroup, four of them (eight
+// gained nothing from 1 x 1024 x 4096 to 16 x 4096 x 16384).  int8, bf16
 // out: 1 x 4096 x 4096 5.8 us (16.8 MB), 64 rows over 64 experts of
 // 1536 x 2048 24 us (about 40 of them have rows: 126 MB, 5.2 TB/s).
 template <bool F8, bool ODD, int MI, int NJ, int WK, int U>
@@ -1084,7 +1085,7 @@ hipError_t launch_linear_any(const LinearArgs& a, bool dma, hipStream_t s) {
     return a.cut ? launch_best_tile<kF8Cut>(a, dma, s) : launch_best_tile<kF8>(a, dma, s);
   }
   if (rows <= 16.f || wgs(16) <= 2.f * cus)
-    return a.K < 8192 ? launch_direct<F8, 1, 1, 4, 4>(a, s) : launch_direct<F8, 1, 1, 8, 4>(a, s);
+    return launch_direct<F8, 1, 1, 4, 4>(a, s);
   return wgs(64) < cus ? launch_direct<F8, 2, 2, 4, 4>(a, s) : launch_direct<F8, 4, 4, 4, 2>(a, s);
 }
 
