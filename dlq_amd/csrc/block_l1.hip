@@ -288,8 +288,8 @@ __global__ __launch_bounds__(512, 1) void block_l1_kernel(BlockArgs a) {
   // Epilogue of one 32 oc x 32 px tile in the MFMA layout (lane: pixel lr,
   // channels h*32 + 8g + 4lh + e) -> 16 contiguous channels (h*32 + 16lh ..)
   // of the pixel.  rs: the residual's 16 bytes in that store layout (conv2).
-  // Pairs of elements go through v_pk_fma_f32 / v_pk_add_f32 (per-component
-  // IEEE fma / add: bit-identical to the scalar sequence).
+  // Elements are written in pairs; the library is built without packed fp32
+  // instructions, so each pair is two scalar fmas / adds (the same IEEE steps).
   auto epilogue = [&](const Acc& acc, bool res, v4i rs) -> v4i {
     if constexpr (F8) {
       unsigned rg[4] = {0, 0, 0, 0};

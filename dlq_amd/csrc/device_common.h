@@ -124,8 +124,9 @@ __device__ __forceinline__ unsigned enc4_f8(float y0, float y1, float y2, float 
   return (unsigned)r;
 }
 
-// e4m3 twins of epi4 / epi4_res on fp32 accumulators (packed fmas, then
-// enc4_f8): per element the same IEEE sequence as the generic fp8 kernel.
+// e4m3 twins of epi4 / epi4_res on fp32 accumulators (fmas written in pairs,
+// issued one by one: the library is built without packed fp32 instructions;
+// then enc4_f8): per element the same IEEE sequence as the generic fp8 kernel.
 __device__ __forceinline__ unsigned epi4_f8(const float* acc, const float* al, const float* be, float lo) {
   const v2f y01 = __builtin_elementwise_fma(v2f{acc[0], acc[1]}, v2f{al[0], al[1]}, v2f{be[0], be[1]});
   const v2f y23 = __builtin_elementwise_fma(v2f{acc[2], acc[3]}, v2f{al[2], al[3]}, v2f{be[2], be[3]});

@@ -518,12 +518,13 @@ __global__ __launch_bounds__(SNW * 64, 4) void stem_fused_kernel(StemArgs a) {
 // row and channel where two lanes issued a ds_write_b16 each.  Same item
 // walk, ring, band logic, pooling and numerics as stem_fused_kernel:
 // 61.5-62.8 -> 59.2-60.6 us per launch (four A/B rounds, one box, round 4),
-// bit-identical.  Round 6 cut its loop from ~197 to 160 non-MFMA VALU per
-// step (24 MFMAs): packed multiply / add in the input conversion, packed fma
-// in the requantisation, the pool pad as a min against a per-lane bound, one
-// permlane32 swap without copies, no result selects in the store -- time
-// unchanged (57.02 vs 57.09 us, profiles/r06_ab_stem_valu.txt): the stem is
-// not bound by VALU issue.
+// bit-identical.  Its loop once went from ~197 to 160 non-MFMA VALU per step
+// (24 MFMAs) -- packed multiply / add in the input conversion, packed fma in
+// the requantisation, the pool pad as a min against a per-lane bound, one
+// permlane32 swap without copies, no result selects in the store -- with the
+// time unchanged (57.02 vs 57.09 us, profiles/r06_ab_stem_valu.txt): the stem
+// is not bound by VALU issue.  Built without packed fp32 instructions the pairs
+// are two scalar instructions each again, and the forward's time is what it was.
 constexpr int S2W = 4;                          // waves: one per column quarter
 constexpr int STG2 = 64 * 16;                   // per wave: [64 oc][16 px] bytes
 constexpr int OFF_STAGE2 = OFF_CR + CR_SLOTS * CR_ROW;
@@ -620,9 +621,9 @@ __global__ __launch_bounds__(S2W * 64, 2) void stem2_kernel(StemArgs a) {
         v = e == 3 ? sa[(2 * jj + 3) & 7] : v;
         ra[jj][i] = v + 12 - 4 * e;
       }
-    // the scale multiply and the rounding add of a column pair in one packed
-    // instruction each (v_pk_mul_f32 / v_pk_add_f32: the same IEEE products and
-    // sums as two scalar ones), the clamp per value
+    // the scale multiply and the rounding add of a column pair at a time (two
+    // scalar instructions each: the library is built without packed fp32 ones),
+    // the clamp per value
     const F2 inv2 = {a.inv_s, a.inv_s}, mg2 = {12582912.0f, 12582912.0f};
     auto convert_quad = [&](const F2 (&r)[2][3], auto jc) {  // jc = (2k) & 7
       constexpr int J = decltype(jc)::value;
@@ -750,10 +751,9 @@ __global__ __launch_bounds__(S2W * 64, 2) void stem2_kernel(StemArgs a) {
         hpool(c[1][ot], Ho);
         unsigned w[2] = {0u, 0u};
 #pragma unroll
-        // two pooled values per v_pk_fma_f32 (the builtin: an inline-asm form
-        // broadcasting alpha / beta by op_sel saved 4 VGPRs but gave ~25
-        // differing bytes per B = 256 launch from run to run -- a hazard the
-        // compiler does not see through asm; tools/probe/stem_det.py)
+        // two pooled values at a time, two scalar fmas (an inline-asm packed form
+        // broadcasting alpha / beta by op_sel gave ~25 differing bytes per B = 256
+        // launch from run to run; tools/probe/stem_det.py)
         for (int m = 0; m < 8; m += 2) {
           const int v0 = max3i(Hp[ot][m], He[m], Ho[m]), v1 = max3i(Hp[ot][m + 1], He[m + 1], Ho[m + 1]);
           Hp[ot][m] = Ho[m];
