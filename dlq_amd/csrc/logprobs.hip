@@ -10,7 +10,8 @@
 // the sums and the alternatives' bound read a row once.  A row of up to 2048
 // logits is one wave's and one of up to 8192 a workgroup's; both place the
 // alternatives in the same launch.  A longer row gets one workgroup per chunk
-// of 8192 (the split that fills the chip when there are few rows) whose waves
+// of 8192, what its registers hold, however many rows there are (so a few rows
+// do not fill the chip: 4 x 100003 is 52 workgroups on 256 CUs).  Its waves
 // work on their own, without a barrier: each leaves (m, S, T) and the largest
 // logit of every four lanes (128 logits).  A second, small launch joins them in
 // chunk order and reads again only those 128s that hold an alternative.
