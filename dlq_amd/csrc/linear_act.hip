@@ -400,18 +400,18 @@ __global__ __launch_bounds__(WK * 64) void linear_direct_kernel(const LinearArgs
 // Waves own 128 x 128 outputs where there are enough rows and columns: an LDS
 // byte then feeds 64 multiply-adds, and reads and DMA writes take 192 KB of
 // the 256 KB that LDS moves in a stage's 2048 matrix cycles (with 128 x 64
-// per wave: 256 KB, the bound).  8192^3, bf16 out: int8 495 us, 2.22 POPS, the
-// clock at 1.7 GHz by the power limit and the matrix unit busy 55 % of the
-// cycles.  Waves of 64 x 64 (128 x 128 tiles) read
-// LDS for as long as they multiply: 576 us.  The small tiles are bound by what
-// a stage takes from DMA to barrier, so they have more slots and up to 128
-// bytes of K per fragment step.
+// per wave: 256 KB, the bound).  8192^3, bf16 out, calls back to back: int8 466
+// us, 2.36 POPS, with GELU 490 to 530 by the card, the clock at 1.7 GHz by the
+// power limit and the matrix unit busy 53 to 57 % of the cycles.  Waves of
+// 64 x 64 (128 x 128 tiles) read LDS for as long as they multiply: 576 us.  The
+// small tiles are bound by what a stage takes from DMA to barrier, so they have
+// more slots and up to 128 bytes of K per fragment step.
 //
 // e4m3 is widened to bf16 here as well (see Mma), behind the LDS read and while
 // matrix instructions run that do not need the fragment: twice the matrix
-// cycles per code, so 8192^3 takes 765 us, 1.44 PFLOP/s, what a bf16 product
-// of this size reaches.  kF8Cut (the caller's DLQ_FP8_SUMS) takes the fp8
-// instructions, 440 us, and their cut products.
+// cycles per code, so 8192^3 takes 760 to 780 us by the card, 1.4 PFLOP/s, what
+// a bf16 product of this size reaches.  kF8Cut (the caller's DLQ_FP8_SUMS) takes
+// the fp8 instructions, 420 to 440 us, and their cut products.
 enum { kS8, kF8, kF8Cut };
 template <int T, int NV>
 struct TileMma {  // a fragment: NV 16-byte reads, 32 K bytes of a row each
