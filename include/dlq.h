@@ -543,7 +543,7 @@ int dlq_quantize_rows_dyn_f8(const void* x, int x_type, int rows, int cols, int 
 typedef struct dlq_linear_desc {
   int M, N, K;            /* rows of x, rows of w (output columns), contraction */
   int ldx, ldw, ldy, ldr; /* row strides in elements (ldr read if residual)     */
-  int act;                /* DLQ_ACT_*                                          */
+  int act;                /* DLQ_ACT_*, for e4m3 with DLQ_FP8_SUMS added or not */
   int out_type;           /* DLQ_T_F32 or DLQ_T_BF16: y and residual            */
 } dlq_linear_desc;
 

@@ -390,6 +390,27 @@ def test_grouped_last_round_of_tiles(gpu, t, off):
     close(y, *grouped_reference(c, off, t, "none", torch.bfloat16, T))
 
 
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("cut", [False, True], ids=["exact", "cut"])
+@pytest.mark.parametrize("off,N,K", [([0, 700, 700, 1500], 2052, 528), ([3, 40, 900, 1490], 2050, 1041),
+                                     ([0, 1500, 1501, 4300], 4612, 272)])
+def test_grouped_f8_sums(gpu, off, N, K, cut, out):
+    """test_linear_f8_sums by expert, through tiles of every kind."""
+    from dlq_amd import ops
+    rng = np.random.default_rng([N, K])
+    T = off[-1] + 10
+    c = grouped_case(rng, "f8", 3, T, N, K, out, res=N == 2052)
+    y = torch.full((T, N), 3.0, dtype=out, device="cuda")
+    ops.linear_grouped_f8(dev(c["x"]), torch.tensor(off, dtype=torch.int32, device="cuda"), dev(c["w"]), dev(c["xs"]),
+                          dev(c["ws"]), dev(c["bias"]), "silu", dev(c["res"]), out=y, fp8_sums=cut)
+    assert (y[:off[0]] == 3.0).all() and (y[off[-1]:] == 3.0).all()
+    for e in range(3):
+        r = slice(off[e], off[e + 1])
+        if off[e] < off[e + 1]:
+            close(y[r], *sums64(c["x"][r], c["w"][e], c["xs"][r], c["ws"][e], c["bias"][e], "silu",
+                                None if c["res"] is None else c["res"][r], out, cut), f"expert {e}")
+
+
 def test_grouped_offsets_outside(gpu):
     """Offsets beyond the rows are taken as the nearest row; nothing else is touched."""
     from dlq_amd import ops
