@@ -8,6 +8,8 @@
 // operand the rows of x: a lane's four accumulators are then four consecutive
 // n of one row m, so scale, bias and residual come in and y goes out in
 // 4-element vectors.
+#include <climits>
+
 #include "rowops_common.h"
 
 namespace dlq {
@@ -1095,6 +1097,8 @@ int linear_any(const char* who, const dlq_linear_desc* d, int E, const int32_t* 
   const auto bad = [&](const char* what) { return fail(DLQ_ERR_ARG, std::string(who) + ": " + what); };
   if (!d || d->M < 0 || d->N < 0 || d->K < 0) return bad("bad shape");
   if (d->K > 131071) return bad("K above 131071");
+  // a row's or column's number plus a tile's height stays an int, here and in the kernels
+  if (d->M > INT_MAX - 511 || d->N > INT_MAX - 511) return bad("M or N above 2^31 - 512");
   const int act = F8 ? d->act & ~DLQ_FP8_SUMS : d->act;
   if (act < DLQ_ACT_NONE || act > DLQ_ACT_SILU) return bad("bad act");
   if (d->out_type != DLQ_T_F32 && d->out_type != DLQ_T_BF16) return bad("bad out_type");

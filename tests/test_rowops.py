@@ -39,6 +39,15 @@ def test_linear_refuses_bad_desc(fn, bad, word):
 
 
 @pytest.mark.parametrize("fn", FNS + GFNS)
+@pytest.mark.parametrize("size", [2 ** 31 - 511, 2 ** 31 - 1])
+def test_linear_refuses_sizes_next_to_2_31(fn, size):
+    """Row and column numbers of the last tile would not be an int's."""
+    for kw in (dict(M=size), dict(N=size, ldy=size)):
+        rc, msg = linear(fn, desc(**kw), x=None, grouped=(2, P) if fn in GFNS else None)
+        assert rc == 1 and "2^31 - 512" in msg, (rc, msg)
+
+
+@pytest.mark.parametrize("fn", FNS + GFNS)
 def test_linear_refuses_pointers(fn):
     g = (2, P) if fn in GFNS else None
     for kw in (dict(x=None), dict(w=None), dict(ws=None), dict(y=None)):
