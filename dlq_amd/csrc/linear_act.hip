@@ -902,11 +902,17 @@ long row_tiles(const LinearArgs& a, int BM) {
   return t < a.M ? t : a.M;
 }
 
+// workgroups of tiles of tn columns by tm rows, 256 threads each: does a launch take them
+bool tiles_fit(const LinearArgs& a, int tn, int tm) {
+  return grid_fits(row_tiles(a, tm) * ((a.N + tn - 1) / tn), 256);
+}
+
 template <int T, bool REG, int WN, int WM, int NI, int MJ, int NV, int KB, int SLOTS, int WPE>
 hipError_t launch_tile(const LinearArgs& a, hipStream_t s) {
   constexpr int TN = 32 * WN * NI, TM = 32 * WM * MJ;
+  static_assert(WN * WM == 4, "256 threads");
   const long nbn = (a.N + TN - 1) / TN, nbm = row_tiles(a, TM);
-  if (!grid_fits(nbm * nbn, WN * WM * 64)) return hipErrorInvalidValue;
+  if (!tiles_fit(a, TN, TM)) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)(nbm * nbn)), threads(WN * WM * 64);
   if (a.vec && a.res)
     hipLaunchKernelGGL((linear_tile_kernel<T, REG, WN, WM, NI, MJ, NV, KB, SLOTS, WPE, true>), grid, threads, 0, s, a,
@@ -920,9 +926,10 @@ hipError_t launch_tile(const LinearArgs& a, hipStream_t s) {
 template <bool F8, bool ODD, int MI, int NJ, int WK, int U>
 hipError_t launch_direct_as(const LinearArgs& a, hipStream_t s) {
   constexpr int BM = 16 * MI, BN = 16 * NJ;
+  static_assert(WK == 4, "256 threads");
   const long nbn = (a.N + BN - 1) / BN;
   const long mt = row_tiles(a, BM);
-  if (!grid_fits(mt * nbn, WK * 64)) return hipErrorInvalidValue;
+  if (!tiles_fit(a, BN, BM)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL((linear_direct_kernel<F8, ODD, MI, NJ, WK, U>), dim3((unsigned)(mt * nbn)), dim3(WK * 64), 0, s, a,
                      (int)mt);
   return hipGetLastError();
@@ -1011,26 +1018,28 @@ float quarters_cost(const TileCost& t128, float rest, float cus, float k) {
   return __builtin_ceilf(4.f * rest / cus) * (t128.one * k + t128.fixed);
 }
 
-// whole: how many tiles of the best kind's stay whole if the others run in
-// quarters (-1: all)
+// The cheapest of the kinds whose tiles a launch takes.  whole: how many of its
+// tiles stay whole if the others run in quarters (-1: all)
 template <int N>
 int best_tile(const LinearArgs& a, const TileCost (&tiles)[N], int& whole) {
   int best = 0;
-  float least = 0.f;
+  float least = INFINITY;
+  whole = -1;
   const float cus = (float)num_cus(), k = a.K / 1024.f;
   for (int i = 0; i < N; ++i) {
     const TileCost& t = tiles[i];
+    if (!tiles_fit(a, t.tn, t.tm)) continue;
     const float wgs = tiles_of_rows(a, t.tm) * (float)((a.N + t.tn - 1) / t.tn), round = cus * t.per_cu;
     const float rounds = __builtin_floorf(wgs / round), rest = wgs - rounds * round;
     float last = rest <= 0.f ? 0.f : (rest <= cus ? t.one : t.two) * k + t.fixed;
     bool quarters = false;
-    if (t.tn == 256 && rounds > 0.f && rest > 0.f) {
+    if (t.tn == 256 && rounds > 0.f && rest > 0.f && grid_fits(4 * row_tiles(a, 256) * ((a.N + 255) / 256), 256)) {
       const float q = quarters_cost(tiles[1], rest, cus, k);
       quarters = q < last;
       if (quarters) last = q;
     }
     const float c = rounds * (t.two * k + t.fixed) + last;
-    if (i == 0 || c < least) {
+    if (c < least) {
       least = c;
       best = i;
       whole = quarters ? (int)(rounds * round) : -1;
@@ -1044,7 +1053,7 @@ hipError_t launch_quarters(const LinearArgs& a, int whole, hipStream_t s) {
   const long nbn = (a.N + 255) / 256, nbm = row_tiles(a, 256);
   if (whole > nbm * nbn) whole = (int)(nbm * nbn);
   const long grid = whole + 4 * (nbm * nbn - whole);
-  if (!grid_fits(grid, 256)) return hipErrorInvalidValue;
+  if (!grid_fits(grid, 256)) return hipErrorInvalidConfiguration;
   if (a.vec && a.res)
     hipLaunchKernelGGL((linear_tile_quarters_kernel<T, true>), dim3((unsigned)grid), dim3(256), 0, s, a, (int)nbm,
                        (int)nbn, whole);
@@ -1086,8 +1095,7 @@ hipError_t launch_linear_any(const LinearArgs& a, bool dma, hipStream_t s) {
     if constexpr (!F8) return launch_best_tile<kS8>(a, dma, s);
     return a.cut ? launch_best_tile<kF8Cut>(a, dma, s) : launch_best_tile<kF8>(a, dma, s);
   }
-  if (rows <= 16.f || wgs(16) <= 2.f * cus)
-    return launch_direct<F8, 1, 1, 4, 4>(a, s);
+  if ((rows <= 16.f || wgs(16) <= 2.f * cus) && tiles_fit(a, 16, 16)) return launch_direct<F8, 1, 1, 4, 4>(a, s);
   return wgs(64) < cus ? launch_direct<F8, 2, 2, 4, 4>(a, s) : launch_direct<F8, 4, 4, 4, 2>(a, s);
 }
 
@@ -1136,6 +1144,7 @@ int linear_any(const char* who, const dlq_linear_desc* d, int E, const int32_t* 
   a.off = off;
   const bool dma = ((uintptr_t)x | (uintptr_t)w) % 16 == 0 && d->K % 16 == 0 && d->ldx % 16 == 0 && d->ldw % 16 == 0;
   const hipError_t e = launch_linear_any<F8>(a, dma, (hipStream_t)stream);
+  if (e == hipErrorInvalidConfiguration) return bad("more tiles than a launch takes");
   return e == hipSuccess ? DLQ_OK : fail(DLQ_ERR_LAUNCH, std::string(who) + " launch: " + hipGetErrorString(e));
 }
 

@@ -559,7 +559,8 @@ typedef struct dlq_linear_desc {
  * x_scale, bias and residual may be NULL (1, 0, none); w_scale not.
  * w is used as stored: no packing.  residual may be y itself (same ld); any
  * other overlap of y with an input is not allowed.  K <= 131071 (an int32 sum
- * of 2^14-sized products); K = 0 gives acc = 0.  M, N <= 2^31 - 512. */
+ * of 2^14-sized products); K = 0 gives acc = 0.  M, N <= 2^31 - 512; a
+ * product of 2^24 or more tiles of 64 x 64 may be refused. */
 int dlq_linear_act_s8(const dlq_linear_desc* d, const int8_t* x, const float* x_scale, const int8_t* w,
                       const float* w_scale, const float* bias, const void* residual, void* y, void* stream);
 int dlq_linear_act_f8(const dlq_linear_desc* d, const uint8_t* x, const float* x_scale, const uint8_t* w,

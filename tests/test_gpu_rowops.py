@@ -292,6 +292,39 @@ def test_linear_offsets_past_32_bits(gpu, t):
     torch.cuda.empty_cache()
 
 
+def test_linear_more_columns_than_small_tiles(gpu):
+    """2^28 columns and more of one row: more 16 x 16 tiles than a launch takes."""
+    from dlq_amd import ops
+    N = 2 ** 28 + 40
+    w = torch.empty(N, 16, dtype=torch.int8, device="cuda")
+    want = torch.arange(N, dtype=torch.int32, device="cuda") % 251 - 125
+    w.copy_(want[:, None])
+    y = ops.linear_act_s8(torch.ones(1, 16, dtype=torch.int8, device="cuda"), w, None, torch.ones(N, device="cuda"))
+    assert torch.equal(y[0], (16 * want).float())
+    del w, y, want
+    torch.cuda.empty_cache()
+
+
+def test_grouped_more_tiles_than_small_ones(gpu):
+    """The same of 4096 experts with 16 rows each on average."""
+    from dlq_amd import ops
+    E, T, N = 4096, 65536, 32768
+    n = torch.arange(N, dtype=torch.int32, device="cuda")
+    w = torch.empty(E, N, 16, dtype=torch.int8, device="cuda")
+    for e in range(0, E, 256):
+        w[e:e + 256] = ((torch.arange(e, e + 256, dtype=torch.int32, device="cuda")[:, None] + n) % 251 - 125)[..., None]
+    off = torch.arange(E + 1, dtype=torch.int32, device="cuda") * 16
+    off[1::2] += 9
+    y = ops.linear_grouped_s8(torch.ones(T, 16, dtype=torch.int8, device="cuda"), off, w, None,
+                              torch.ones(E, N, device="cuda"), out_dtype=torch.bfloat16)
+    expert = torch.repeat_interleave(torch.arange(E, device="cuda"), (off[1:] - off[:-1]).long()).int()
+    for t in range(0, T, 4096):
+        want = 16 * ((expert[t:t + 4096, None] + n) % 251 - 125)
+        assert torch.equal(y[t:t + 4096], want.bfloat16()), t
+    del w, y, want
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("M,N,K,ldr", [(300, 1700, 192, 1 << 21), (300, 1700, 192, (1 << 21) + 4),
                                        (700, 1028, 192, 1028), (700, 1028, 193, 1032), (700, 1028, 193, 1029),

@@ -77,6 +77,15 @@ def test_fp8_sums_belong_to_e4m3(fn):
         assert rc == 1 and "bad act" in msg
 
 
+@pytest.mark.parametrize("fn", FNS + GFNS)
+def test_linear_refuses_more_tiles_than_a_launch_takes(fn):
+    g = (2, P) if fn in GFNS else None
+    n = 2 ** 31 - 512
+    for kw in (dict(M=n, N=n, ldy=n), dict(M=1, N=n, ldy=n), dict(M=1 << 20, N=n, K=33, ldx=33, ldw=33, ldy=n)):
+        rc, msg = linear(fn, desc(**kw), grouped=g)
+        assert rc == 1 and "more tiles" in msg, (kw, rc, msg)
+
+
 @pytest.mark.parametrize("fn", GFNS)
 def test_grouped_refuses(fn):
     rc, msg = linear(fn, desc(), grouped=(2, None))
