@@ -863,6 +863,9 @@ __global__ __launch_bounds__(WN* WM * 64, WPE) void linear_tile_kernel(const Lin
 // 16-byte reads per fragment.  Widened e4m3 has the shortest in the large tiles:
 // its widening runs behind more matrix instructions then, and spills nothing
 // (8192^3: 760 us, 1020 with two; 128 x 128 tiles of 4096^3 143, 147 with two).
+// A 64 x 64 tile's step has one product per fragment, and takes as long a one as
+// registers allow (32 x 12288 x 4096: 16.4 us with four, 17.5 with two; through
+// registers 4096 x 4096 x 4099 249 with two, 269 with four).
 template <int T>
 constexpr int kNv64 = T == kF8Cut ? 2 : 4;
 template <int T>
@@ -1092,8 +1095,10 @@ hipError_t launch_linear_any(const LinearArgs& a, bool dma, hipStream_t s) {
   const auto wgs = [&](int t) { return tiles_of_rows(a, t) * (float)((a.N + t - 1) / t); };
   // tiles from half as many workgroups as CUs on; their rows' byte offsets are 32 bits
   if (rows > 16.f && wgs(64) >= 0.5f * cus && a.ldx <= (1 << 22) && a.ldw <= (1 << 22) && a.ldr <= (1 << 21)) {
-    if constexpr (!F8) return launch_best_tile<kS8>(a, dma, s);
-    return a.cut ? launch_best_tile<kF8Cut>(a, dma, s) : launch_best_tile<kF8>(a, dma, s);
+    if constexpr (!F8)
+      return launch_best_tile<kS8>(a, dma, s);
+    else
+      return a.cut ? launch_best_tile<kF8Cut>(a, dma, s) : launch_best_tile<kF8>(a, dma, s);
   }
   if ((rows <= 16.f || wgs(16) <= 2.f * cus) && tiles_fit(a, 16, 16)) return launch_direct<F8, 1, 1, 4, 4>(a, s);
   return wgs(64) < cus ? launch_direct<F8, 2, 2, 4, 4>(a, s) : launch_direct<F8, 4, 4, 4, 2>(a, s);
